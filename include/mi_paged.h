@@ -96,6 +96,22 @@ int mi_kv_gather_blocks(const void* pool, const int64_t* block_ids, int64_t batc
                         void* stream);
 
 /*
+ * mi_kv_copy_blocks — copy whole blocks inside every one of num_pools pools (each layer's K and V):
+ * pools[i][dst] = pools[i][src] for every pair (src, dst), in one launch.  For a forked sequence's
+ * private copy of a partly filled block and for compaction (no counterpart in the reference, whose
+ * blocks belong to one sequence).  The bytes are copied as they are, so the pools may hold any
+ * element type, 4-bit pages (mi_kv4.h) among them.
+ *   pools   [num_pools] device pointers in host memory, read before the call returns
+ *   pairs   [num_pairs, 2] int64 (src, dst) on the device.  Destinations must be distinct and no
+ *           destination may be a source of another pair (nothing orders the pairs); a pair with
+ *           src == dst does nothing.  A pair with an id outside [0, num_blocks) is skipped and sets
+ *           MI_STATUS_BAD_BLOCK.
+ *   block_bytes  bytes of one block of one pool
+ */
+int mi_kv_copy_blocks(void* const* pools, int num_pools, const int64_t* pairs, int64_t num_pairs,
+                      int64_t num_blocks, int64_t block_bytes, void* stream);
+
+/*
  * mi_paged_decode — one decode step of paged GQA attention for one layer (one query token per
  * sequence).  Replaces the history gather + _attend of the paged branch
  * (model/qwen3.py:285-292 and :219-255, bias of :513-527): sequence b attends to positions

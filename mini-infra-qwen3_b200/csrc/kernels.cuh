@@ -214,4 +214,92 @@ struct SiluMulArgs {
 };
 cudaError_t launch_silu_mul(const SiluMulArgs& a, bool vec16, int dtype, cudaStream_t s);
 
+// ------------------------------------------------------------------------------------------
+// 4-bit paged cache (kv4_format.cuh) and block copies
+// ------------------------------------------------------------------------------------------
+struct Kv4StoreArgs {
+  const char* k_src;
+  const char* v_src;
+  int64_t k_sb[3];  // row, head, position
+  int64_t v_sb[3];
+  // tokens at given slots
+  const int64_t* rows;       // may be null: row = token index
+  const int64_t* positions;  // may be null: position 0
+  const int64_t* slots;
+  int64_t num_tokens;
+  int64_t src_rows;
+  int64_t src_positions;
+  // right-aligned chunks through block tables
+  int64_t batch;
+  int64_t padded_len;
+  const int64_t* chunk_lens;
+  const int64_t* starts;
+  const int64_t* block_tables;
+  int64_t table_stride;
+  int64_t table_width;
+  char* k_pool;
+  char* v_pool;
+  int64_t num_blocks;
+  int64_t page_bytes;
+  int block_size;
+  int heads;
+  int head_dim;
+};
+cudaError_t launch_kv4_store(const Kv4StoreArgs& a, bool chunks, bool vec, int dtype, cudaStream_t s);
+
+struct Kv4GatherArgs {
+  const char* k_pool;
+  const char* v_pool;
+  const int64_t* block_ids;
+  int64_t id_stride;
+  const int64_t* lengths;  // may be null: every token
+  int64_t batch;
+  int64_t blocks_per_row;
+  char* k_out;
+  char* v_out;
+  int64_t num_blocks;
+  int64_t page_bytes;
+  int block_size;
+  int heads;
+  int head_dim;
+};
+cudaError_t launch_kv4_gather(const Kv4GatherArgs& a, int dtype, cudaStream_t s);
+
+struct Kv4DecodeArgs {
+  const char* q;
+  int64_t q_sb, q_sh;  // bytes
+  const char* k_pool;
+  const char* v_pool;
+  int64_t page_bytes;
+  const int64_t* block_tables;
+  int64_t table_stride;
+  int64_t max_blocks;
+  const int64_t* context_lens;
+  int64_t batch;
+  int64_t num_blocks;
+  int hq, hkv, groups;
+  int head_dim;
+  int block_size;
+  float scale_log2;
+  char* out;
+  int64_t out_sb;  // bytes
+};
+struct Kv4DecodePlan {
+  size_t ws_bytes;
+};
+Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int64_t max_blocks, int block_size,
+                              int dtype);
+cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const Kv4DecodePlan& plan, int dtype, cudaStream_t s);
+
+constexpr int kMaxCopyPools = 128;  // pools of one launch
+struct PageCopyArgs {
+  char* pools[kMaxCopyPools];
+  const int64_t* pairs;
+  int64_t num_pairs;
+  int64_t num_blocks;
+  int64_t block_bytes;
+  int num_pools;
+};
+cudaError_t launch_page_copy(const PageCopyArgs& a, int vec_bytes, cudaStream_t s);
+
 }  // namespace mi

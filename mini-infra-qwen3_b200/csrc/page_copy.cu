@@ -1,0 +1,46 @@
+// Whole blocks copied inside every pool of the cache: (src, dst) pairs x pools in one launch.
+//
+// Pure data movement, 2 * block_bytes of HBM traffic per pair and pool.  One CTA per (pair, pool).
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace mi {
+namespace {
+
+constexpr int kPageCopyThreads = 256;
+
+template <typename V>
+__global__ void __launch_bounds__(kPageCopyThreads) page_copy_kernel(const __grid_constant__ PageCopyArgs a) {
+  const int64_t pair = blockIdx.x;
+  const int64_t src = a.pairs[2 * pair], dst = a.pairs[2 * pair + 1];
+  if (src < 0 || src >= a.num_blocks || dst < 0 || dst >= a.num_blocks) {
+    if (threadIdx.x == 0) record_status(MI_STATUS_BAD_BLOCK);
+    return;
+  }
+  if (src == dst) return;
+  char* pool = a.pools[blockIdx.y];
+  const int64_t units = a.block_bytes / (int64_t)sizeof(V);
+  const V* from = reinterpret_cast<const V*>(pool + src * a.block_bytes);
+  V* to = reinterpret_cast<V*>(pool + dst * a.block_bytes);
+  for (int64_t i = threadIdx.x; i < units; i += kPageCopyThreads) to[i] = __ldg(from + i);
+}
+
+template <typename V>
+cudaError_t launch_page_copy_t(const PageCopyArgs& a, cudaStream_t s) {
+  page_copy_kernel<V><<<dim3((unsigned)a.num_pairs, (unsigned)a.num_pools), kPageCopyThreads, 0, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_page_copy(const PageCopyArgs& a, int vec_bytes, cudaStream_t s) {
+  switch (vec_bytes) {
+    case 16: return launch_page_copy_t<uint4>(a, s);
+    case 8: return launch_page_copy_t<uint2>(a, s);
+    case 4: return launch_page_copy_t<uint32_t>(a, s);
+    case 2: return launch_page_copy_t<uint16_t>(a, s);
+    default: return launch_page_copy_t<uint8_t>(a, s);
+  }
+}
+
+}  // namespace mi

@@ -1,4 +1,4 @@
-"""ctypes binding of libmi_paged.so (the C ABI declared in include/mi_paged.h).
+"""ctypes binding of libmi_paged.so (the C ABI declared in include/*.h).
 
 The library is loaded lazily on first use and must exist: there is no fallback of any kind.  A
 missing library raises ``RuntimeError`` naming the build command.  Every wrapper checks the
@@ -54,7 +54,19 @@ SIGNATURES: dict[str, tuple] = {
         [_P, _I64P, _P, _P, _I64P, _P, _P, _L, _I, _I, _I, _P, _L, _P, _P, _L, _L, _I, ctypes.c_float, _P, _P,
          ctypes.c_size_t, _I, _P],
     ),
+    "mi_kv_copy_blocks": (_I, [_P, _I, _P, _L, _L, _L, _P]),
     "mi_decode_rows": (_I, [_P, _L, _P, _L, _P, _L, _L, _P, _L, _L, _I, _P]),
+    # include/mi_kv4.h
+    "mi_kv4_page_bytes": (_L, [_I, _I]),
+    "mi_kv4_scatter": (_I, [_P, _P, _I64P, _I64P, _L, _L, _P, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "mi_kv4_store_chunks": (_I, [_P, _P, _I64P, _I64P, _L, _L, _P, _P, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "mi_kv4_gather_blocks": (_I, [_P, _P, _P, _L, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "mi_kv4_paged_decode_workspace_size": (ctypes.c_size_t, [_L, _I, _I, _I, _L, _I, _I]),
+    "mi_kv4_paged_decode": (
+        _I,
+        [_P, _I64P, _P, _P, _I64P, _P, _P, _P, _L, _I, _I, _I, _P, _L, _L, _P, _L, _I, ctypes.c_float, _P, _L, _P,
+         ctypes.c_size_t, _I, _P],
+    ),
     # include/mi_layers.h
     "mi_rmsnorm": (_I, [_P, _L, _P, _L, _P, _L, _P, _P, _L, _L, _I, ctypes.c_float, _I, _P]),
     "mi_qk_norm_rope": (

@@ -8,7 +8,9 @@ per-device buffer that grows on demand (the library itself never allocates).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
+from collections.abc import Sequence
 
 import torch
 
@@ -491,4 +493,244 @@ def decode_rows(
         _ptr(rows), rows.numel() // 3, _ptr(deltas if nd else None), nd, _ptr(tables), tables.shape[0],
         tables.shape[1], _ptr(out), n, width, block_size, _stream(device))
     nat.check(rc, "mi_decode_rows")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# Block copies and the 4-bit paged cache (include/mi_kv4.h).  These run on the current stream of
+# the tensors' device, which need not be the current device; their workspaces come from PyTorch's
+# allocator at each call, so calls on different streams and captured graphs share none.
+# ---------------------------------------------------------------------------------------------
+KV4_GROUP = 32  # values along head_dim that share a step and a minimum
+
+
+def _on(device: torch.device):
+    """A context with `device` current (launches go to the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def kv_copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
+    """pool[dst] = pool[src] in every pool for every (src, dst) row of `pairs` [n, 2] int64, in one launch.
+
+    pools: contiguous tensors of the same number and size of blocks (their first dimension), of any
+    type, 4-bit pages among them.  Destinations must be distinct and not be sources of other pairs
+    (nothing orders the pairs; ``PagedKVCachePool.copy_blocks`` checks that); (b, b) does nothing.
+    Ids out of range are skipped and set MI_STATUS_BAD_BLOCK."""
+    device = _require_cuda("kv_copy_blocks", pairs, *pools)
+    if not pools:
+        return
+    blocks, size = pools[0].shape[0] if pools[0].ndim else 0, pools[0].nbytes
+    for p in pools:
+        if p.ndim < 2 or p.shape[0] != blocks or p.nbytes != size or not p.is_contiguous():
+            raise ValueError("pools must be contiguous [num_blocks, ...] tensors of the same blocks and bytes")
+    pairs = _index(pairs, "pairs")
+    if pairs.ndim != 2 or pairs.shape[1] != 2:
+        raise ValueError(f"pairs must be [n, 2], got {tuple(pairs.shape)}")
+    if blocks == 0 or size == 0:
+        return
+    table = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    with _on(device):
+        rc = nat.load().mi_kv_copy_blocks(table, len(pools), _ptr(pairs), pairs.shape[0], blocks, size // blocks,
+                                          _stream(device))
+    nat.check(rc, "mi_kv_copy_blocks")
+
+
+def kv4_page_bytes(block_size: int, head_dim: int) -> int:
+    """Bytes of one 4-bit page: `block_size` tokens of one KV head (5 bits a value)."""
+    if block_size < 1 or head_dim % KV4_GROUP or not KV4_GROUP <= head_dim <= 256:
+        raise ValueError(f"a 4-bit cache needs a positive block_size and head_dim a multiple of {KV4_GROUP} up to 256 "
+                         f"(got {block_size}, {head_dim})")
+    return block_size * head_dim * 5 // 8
+
+
+def _check_kv4(k_pool: torch.Tensor, v_pool: torch.Tensor, head_dim: int) -> tuple[int, int, int]:
+    """(num_blocks, block_size, num_kv_heads) of 4-bit pools for this head_dim."""
+    if (k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or k_pool.ndim != 3 or k_pool.shape != v_pool.shape
+            or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
+        raise ValueError(f"4-bit pools must be contiguous uint8 [num_blocks, num_kv_heads, page bytes], got "
+                         f"{tuple(k_pool.shape)} {k_pool.dtype} / {tuple(v_pool.shape)} {v_pool.dtype}")
+    n, h, page = k_pool.shape
+    bs = page // kv4_page_bytes(1, head_dim)
+    if bs < 1 or bs * kv4_page_bytes(1, head_dim) != page:
+        raise ValueError(f"pages of {page} bytes hold no whole number of tokens of head_dim {head_dim}")
+    return n, bs, h
+
+
+def kv4_scatter(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    token_rows: torch.Tensor | None,
+    token_positions: torch.Tensor | None,
+    slot_mapping: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+) -> None:
+    """``kv_scatter`` into 4-bit pools: token i = src[token_rows[i], :, token_positions[i], :] of K and V is
+    quantised into slot slot_mapping[i].  key/value: [B, H, L, D], or [B, H, D] with both index tensors None."""
+    device = _require_cuda("kv4_scatter", key, value, slot_mapping, k_pool, v_pool, token_rows, token_positions)
+    if key.shape != value.shape or key.ndim not in (3, 4) or key.dtype != value.dtype:
+        raise ValueError(f"key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} must be "
+                         "[B, H, L, D] or [B, H, D] alike")
+    d = key.shape[-1]
+    n, bs, h = _check_kv4(k_pool, v_pool, d)
+    if key.shape[1] != h:
+        raise ValueError(f"source {tuple(key.shape)} does not match the pools' {h} heads")
+    key, value = _rows_contiguous_last(key), _rows_contiguous_last(value)
+    ks, vs = key.stride(), value.stride()
+    if key.ndim == 3:
+        if token_rows is not None or token_positions is not None:
+            raise ValueError("a [B, H, D] source takes no token_rows/token_positions")
+        ks, vs, src_positions = (ks[0], ks[1], 0), (vs[0], vs[1], 0), 1
+    else:
+        ks, vs, src_positions = ks[:3], vs[:3], key.shape[2]
+    slots = _index(slot_mapping, "slot_mapping")
+    rows = _index(token_rows, "token_rows") if token_rows is not None else None
+    positions = _index(token_positions, "token_positions") if token_positions is not None else None
+    for name, t in (("token_rows", rows), ("token_positions", positions)):
+        if t is not None and t.numel() != slots.numel():
+            raise ValueError(f"{name} has {t.numel()} entries, slot_mapping {slots.numel()}")
+    if rows is None and slots.numel() > key.shape[0]:
+        raise ValueError(f"{slots.numel()} slots for a source of {key.shape[0]} rows")
+    with _on(device):
+        rc = nat.load().mi_kv4_scatter(
+            _ptr(key), _ptr(value), nat.i64_array(ks), nat.i64_array(vs), key.shape[0], src_positions, _ptr(rows),
+            _ptr(positions), _ptr(slots), slots.numel(), _ptr(k_pool), _ptr(v_pool), n, bs, h, d,
+            dtype_code(key.dtype), _stream(device))
+    nat.check(rc, "mi_kv4_scatter")
+
+
+def kv4_store_chunks(
+    key: torch.Tensor,
+    value: torch.Tensor,
+    chunk_lens: torch.Tensor,
+    start_positions: torch.Tensor,
+    block_tables: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+) -> None:
+    """``kv_store_chunks`` into 4-bit pools: each row's right-aligned chunk tokens (key/value [B, H, L, D]) are
+    quantised at their table slots."""
+    device = _require_cuda("kv4_store_chunks", key, value, chunk_lens, start_positions, block_tables, k_pool, v_pool)
+    if key.shape != value.shape or key.ndim != 4 or key.dtype != value.dtype:
+        raise ValueError(f"key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} must be "
+                         "[B, H, L, D] alike")
+    b, heads, length, d = key.shape
+    n, bs, h = _check_kv4(k_pool, v_pool, d)
+    if heads != h:
+        raise ValueError(f"source {tuple(key.shape)} does not match the pools' {h} heads")
+    key, value = _rows_contiguous_last(key), _rows_contiguous_last(value)
+    tables, lens = _index(block_tables, "block_tables"), _index(chunk_lens, "chunk_lens")
+    starts = _index(start_positions, "start_positions")
+    if lens.numel() != b or starts.numel() != b or tables.ndim != 2 or tables.shape[0] != b:
+        raise ValueError("chunk_lens, start_positions and block_tables need one row per batch row")
+    with _on(device):
+        rc = nat.load().mi_kv4_store_chunks(
+            _ptr(key), _ptr(value), nat.i64_array(key.stride()[:3]), nat.i64_array(value.stride()[:3]), b, length,
+            _ptr(lens), _ptr(starts), _ptr(tables), tables.shape[1], tables.shape[1], _ptr(k_pool), _ptr(v_pool), n,
+            bs, h, d, dtype_code(key.dtype), _stream(device))
+    nat.check(rc, "mi_kv4_store_chunks")
+
+
+def kv4_gather_blocks(
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_ids: torch.Tensor,
+    head_dim: int,
+    dtype: torch.dtype,
+    lengths: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Blocks of 4-bit pools as dense ones: (key, value), each [B, nb, bs, H, D] in `dtype` for block_ids
+    [B, nb].  With lengths [B], row b's tokens at and past lengths[b] are zeros and the ids of blocks past
+    it are not read."""
+    device = _require_cuda("kv4_gather_blocks", k_pool, v_pool, block_ids, lengths)
+    n, bs, h = _check_kv4(k_pool, v_pool, head_dim)
+    if block_ids.dtype != torch.int64 or block_ids.ndim != 2:
+        raise ValueError(f"block_ids must be int64 [B, blocks], got {tuple(block_ids.shape)} {block_ids.dtype}")
+    ids = block_ids if block_ids.stride(-1) == 1 or block_ids.shape[1] <= 1 else block_ids.contiguous()
+    b, nb = ids.shape
+    if lengths is not None:
+        lengths = _index(lengths, "lengths")
+        if lengths.numel() != b:
+            raise ValueError(f"lengths has {lengths.numel()} entries for {b} rows")
+    code = dtype_code(dtype)
+    key = torch.empty((b, nb, bs, h, head_dim), dtype=dtype, device=device)
+    value = torch.empty_like(key)
+    with _on(device):
+        rc = nat.load().mi_kv4_gather_blocks(
+            _ptr(k_pool), _ptr(v_pool), _ptr(ids), ids.stride(0) if b > 1 else nb, _ptr(lengths), b, nb, _ptr(key),
+            _ptr(value), n, bs, h, head_dim, code, _stream(device))
+    nat.check(rc, "mi_kv4_gather_blocks")
+    return key, value
+
+
+def kv4_paged_decode(
+    query: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    scale: float,
+    key_new: torch.Tensor | None = None,
+    value_new: torch.Tensor | None = None,
+    slot_mapping: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    ws: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``paged_decode`` over 4-bit pools: query [B, Hq, D] -> out [B, Hq * D] in the query's type.
+
+    With key_new/value_new/slot_mapping the new token's K/V ([B, H, D]) are quantised into the pools
+    first, so that the row attends to them as the cache holds them."""
+    device = _require_cuda("kv4_paged_decode", query, k_pool, v_pool, block_tables, context_lens, key_new, value_new,
+                           slot_mapping, out, ws)
+    if query.ndim != 3:
+        raise ValueError(f"query must be [B, Hq, D], got {tuple(query.shape)}")
+    b, hq, d = query.shape
+    n, bs, h = _check_kv4(k_pool, v_pool, d)
+    code = dtype_code(query.dtype)
+    query = _rows_contiguous_last(query)
+    if block_tables.dtype != torch.int64 or block_tables.ndim != 2 or block_tables.shape[0] != b:
+        raise ValueError(f"block_tables must be int64 [B, max_blocks], got {tuple(block_tables.shape)} "
+                         f"{block_tables.dtype}")
+    width = block_tables.shape[1]
+    tables = block_tables if block_tables.stride(-1) == 1 or width <= 1 else block_tables.contiguous()
+    ctx = _index(context_lens, "context_lens")
+    if ctx.numel() != b:
+        raise ValueError(f"context_lens has {ctx.numel()} entries for batch {b}")
+    if hq < 1 or hq % h:
+        raise ValueError(f"{hq} query heads are not a multiple of {h} KV heads")
+    new_strides = None
+    if (key_new is None) != (value_new is None) or (key_new is None) != (slot_mapping is None):
+        raise ValueError("key_new, value_new and slot_mapping go together")
+    if key_new is not None:
+        if (key_new.shape != (b, h, d) or value_new.shape != (b, h, d) or slot_mapping.numel() != b
+                or key_new.dtype != query.dtype or value_new.dtype != query.dtype):
+            raise ValueError(f"key_new/value_new must be [{b}, {h}, {d}] {query.dtype} with one slot per row")
+        key_new, value_new = _rows_contiguous_last(key_new), _rows_contiguous_last(value_new)
+        if key_new.stride() != value_new.stride():
+            key_new, value_new = key_new.contiguous(), value_new.contiguous()
+        new_strides = nat.i64_array(key_new.stride()[:2])
+        slot_mapping = _index(slot_mapping, "slot_mapping")
+    if out is None:
+        out = torch.empty((b, hq * d), dtype=query.dtype, device=device)
+    elif out.shape != (b, hq * d) or out.dtype != query.dtype or out.stride(-1) != 1:
+        raise ValueError(f"out must be [{b}, {hq * d}] {query.dtype} with contiguous rows")
+    if b == 0:
+        return out
+    lib = nat.load()
+    need = int(lib.mi_kv4_paged_decode_workspace_size(b, hq, h, d, width, bs, code))
+    base, avail = None, 0
+    if need:
+        if ws is None:
+            ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
+        base = (ws.data_ptr() + 255) & ~255
+        avail = ws.nbytes - (base - ws.data_ptr())
+    with _on(device):
+        rc = lib.mi_kv4_paged_decode(
+            _ptr(query), nat.i64_array(query.stride()[:2]), _ptr(key_new), _ptr(value_new), new_strides,
+            _ptr(slot_mapping), _ptr(k_pool), _ptr(v_pool), n, bs, h, d, _ptr(tables),
+            tables.stride(0) if b > 1 else width, width, _ptr(ctx), b, hq, float(scale), _ptr(out), out.stride(0), base,
+            avail, code, _stream(device))
+    nat.check(rc, "mi_kv4_paged_decode")
     return out
