@@ -175,8 +175,10 @@ int mi_kv4_paged_decode(const void* q, const int64_t* q_strides, const void* k_n
                 (long long)max_blocks_per_seq, (long long)table_stride);
   const int es = elem_size(dtype);
   if (!aligned(q, es) || !aligned(out, es)) return fail(MI_ERR_INVALID, "mi_kv4_paged_decode: misaligned operands");
-  const mi::Kv4DecodePlan plan =
+  mi::Kv4DecodePlan plan =
       mi::plan_kv4_decode(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq, block_size, dtype);
+  // the tensor-core kernel copies 16-byte aligned pages; head_dim >= 64 makes every page a multiple of 16
+  if (plan.use_mma && !(aligned(k_pool, 16) && aligned(v_pool, 16))) plan = mi::Kv4DecodePlan{};
   if (plan.ws_bytes && (!workspace || workspace_bytes < plan.ws_bytes || !aligned(workspace, 256)))
     return fail(MI_ERR_INVALID, "workspace must be >= %zu bytes and 256-byte aligned (got %zu)", plan.ws_bytes,
                 workspace_bytes);
@@ -209,6 +211,14 @@ int mi_kv4_paged_decode(const void* q, const int64_t* q_strides, const void* k_n
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<char*>(out);
   a.out_sb = out_stride * es;
+  a.split_pages = plan.split_pages;
+  a.max_splits = plan.max_splits;
+  a.max_parts = plan.max_splits * plan.parts_per_split;
+  if (plan.ws_bytes) {
+    const size_t o_bytes = (size_t)batch * num_q_heads * a.max_parts * head_dim * sizeof(float);
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((o_bytes + 255) & ~size_t(255)));
+  }
   cudaError_t e = mi::launch_kv4_decode(a, plan, dtype, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MI_OK : cuda_fail(e, "mi_kv4_paged_decode launch");
 }

@@ -283,8 +283,19 @@ struct Kv4DecodeArgs {
   float scale_log2;
   char* out;
   int64_t out_sb;  // bytes
+  // tensor-core path
+  int split_pages;  // pages handled by one split
+  int max_splits;   // grid.x
+  int max_parts;    // partials of one row: max_splits * parts_per_split
+  float* ws_o;      // [batch, hq, max_parts, head_dim]
+  float* ws_ml;     // [batch, hq, max_parts, 2]
 };
 struct Kv4DecodePlan {
+  bool use_mma;
+  int heads_per_cta;
+  int parts_per_split;
+  int split_pages;
+  int max_splits;
   size_t ws_bytes;
 };
 Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int64_t max_blocks, int block_size,

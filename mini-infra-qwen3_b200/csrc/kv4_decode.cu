@@ -3,10 +3,32 @@
 // A row's output is sum_t p_t v_t / sum_t p_t, p_t = exp(scale * q.k_t), k_t and v_t the values their
 // codes stand for.
 //
+// Tensor-core kernel (16-bit types, head_dim 64/128, block size 16/32, at most 8 query heads per KV
+// head).  With k = m + s c per group g of 32 values,
+//     q.k_t = sum_g s_tg (q_g . c_tg) + m_tg sum(q_g),     o = sum_t (p_t s_tg) c_tg + p_t m_tg,
+// so the codes themselves are the MMA operands and the steps and minima enter once per token and group:
+// there is no pass that dequantises.  A code is masked out of its word straight into a half: c in bits
+// 0-3 of a half is the subnormal c * 2^-24, in bits 4-7 it is 16 c * 2^-24, both exact, so one AND makes
+// two operands and one shift serves eight codes.  The 16s go into q (K) and into the epilogue (V).
+//   * Tokens are the M rows of S^T = K Q^T (m16n8k16, N = up to 8 query heads), head_dim values those of
+//     O^T = V^T P^T; the transposed orientation fills all 16 rows where the query heads would fill at
+//     most 8.  P^T gets from accumulator to operand layout by movmatrix, once per group of 32 values
+//     because p s differs by group.
+//   * q is scaled by a power of two to a largest value in [2^14, 2^15) and held in fp16: exact for the
+//     16-bit types except far below the row's largest value (absolute error 2^-24 of it).
+//   * p s is held in fp16.  The running reference of the softmax is that of p * s (see kv4_reference):
+//     products lie in fp16's upper range, rounding them costs 2^-12 of a weight; an fp16 model, whose
+//     output has as many bits, carries the rounding's remainder in a second fp16 operand.
+//   * Scores, sums, the minimum terms and O are fp32.
+// grid = (splits, KV head blocks, batch); a producer warp brings whole pages (all heads of the block in
+// one bulk copy for K and one for V) into a ring of shared-memory stages, 4 consumer warps each take a
+// (KV head, page) of a stage.  The splits' partials are merged by decode_combine_kernel.
+//
 // Generic kernel (any type, head_dim, block size and group count): one CTA per (sequence, query head);
 // its warps take the pages in turn, a lane holding value lane of every group, with an online softmax in
 // fp32, and merge in shared memory.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.cuh"
@@ -96,16 +118,442 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_decode_generic_kernel(cons
   dst[d] = Elem<T>::from_f(l == 0.f ? 0.f : o / l);
 }
 
+constexpr int kKv4Consumers = 4;  // consumer warps of the tensor-core kernel's CTA
+constexpr int kKv4SplitThreads = (kKv4Consumers + 1) * 32;
+constexpr int kKv4Smem = 62 * 1024;  // three CTAs per SM
+
+template <int D, int BS, int HB>
+struct Kv4Shape {
+  static constexpr int kGroups = D / kKv4Group;
+  static constexpr int kPages = kKv4Consumers / HB;  // pages of a stage: one (KV head, page) per warp
+  static constexpr int kPageBytes = BS * D / 2 + BS * kGroups * 4;
+  static constexpr int kStageBytes = kPages * HB * 2 * kPageBytes;
+  static constexpr int kStages = std::max(2, std::min(8, kKv4Smem / kStageBytes));
+  static constexpr int kSmemBytes = kStages * (kStageBytes + 16) + 128;
+};
+
+constexpr float kKv4TopLog2 = 11.f;    // p * s of a new reference: at most 2^11
+constexpr float kKv4Limit = 32768.f;   // p * s above this moves the reference (fp16 ends at 65504)
+constexpr float kKv4PLog2 = 60.f;      // p alone of a new reference: at most 2^60
+constexpr float kKv4PLimit = 0x1p68f;
+
+__device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }  // -126 <= n <= 128
+
+// The reference a token asks for: weights are exp2(x - reference), x the score in powers of two, so
+// that p * s <= 2^11 for its widest step s, and p <= 2^60 where the steps are (nearly) zero.
+__device__ __forceinline__ float kv4_reference(float x, float widest) {
+  return x + fmaxf(log2f(widest) - kKv4TopLog2, -kKv4PLog2);
+}
+
+// Four operands out of eight codes: codes (0, 4), (1, 5) times 16, (2, 6), (3, 7) times 16, as halves
+// in units of 2^-24.
+__device__ __forceinline__ void kv4_operands(uint32_t w, uint32_t (&o)[4]) {
+  o[0] = w & 0x000f000fu;
+  o[1] = w & 0x00f000f0u;
+  const uint32_t w8 = w >> 8;
+  o[2] = w8 & 0x000f000fu;
+  o[3] = w8 & 0x00f000f0u;
+}
+
+template <int NG>
+__device__ __forceinline__ void kv4_params(const uint8_t* p, uint32_t (&w)[NG]) {
+  if constexpr (NG == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x, w[1] = u.y;
+  }
+}
+
+template <typename T, int D, int BS, int HB>
+__global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(const Kv4DecodeArgs a) {
+  using S = Kv4Shape<D, BS, HB>;
+  constexpr int NG = S::kGroups;
+  constexpr int NST = S::kStages;
+  constexpr int PG = S::kPages;
+  constexpr bool kTwo = std::is_same<T, __half>::value;  // p * s as two fp16 operands
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the append
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + NST * S::kStageBytes);
+  uint64_t* empty_bar = full_bar + NST;
+
+  const int split = blockIdx.x;
+  const int head0 = blockIdx.y * HB;
+  const int64_t b = blockIdx.z;
+  int64_t ctx = a.context_lens[b];
+  int64_t n_pages = ctx > 0 ? (ctx + BS - 1) / BS : 0;
+  if (n_pages > a.max_blocks) {
+    if (threadIdx.x == 0 && split == 0) record_status(MI_STATUS_BAD_LENGTH);
+    n_pages = a.max_blocks;
+    ctx = n_pages * BS;
+  }
+  const int64_t page_begin = (int64_t)split * a.split_pages;
+  if (page_begin >= n_pages) return;  // uniform for the CTA
+  const int64_t page_end = min(n_pages, page_begin + (int64_t)a.split_pages);
+  const int n_iter = (int)((page_end - page_begin + PG - 1) / PG);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], kKv4Consumers);
+    }
+    fence_mbar_init();
+  }
+  __syncthreads();
+  bool aborted = false;
+
+  if (warp == kKv4Consumers) {
+    // ---------------- producer: lane 2p + kv copies K or V of page p of a stage ----------------
+    constexpr uint32_t kBytes = HB * S::kPageBytes;
+    const int my_page = lane >> 1;
+    const bool mine = my_page < PG;
+    const char* pool = ((lane & 1) ? a.v_pool : a.k_pool) + (int64_t)head0 * S::kPageBytes;
+    const int64_t block_bytes = (int64_t)a.hkv * S::kPageBytes;
+    const int64_t* table = a.block_tables + b * a.table_stride;
+    int64_t next_blk = 0;  // each lane reads its next block id one stage ahead
+    if (mine && page_begin + my_page < page_end) next_blk = table[page_begin + my_page];
+    for (int it = 0; it < n_iter; ++it) {
+      const int st = it % NST;
+      if (it >= NST) {
+        mbar_wait(&empty_bar[st], ((it / NST) - 1) & 1, aborted);
+        aborted = __any_sync(0xffffffffu, aborted);
+      }
+      const int64_t first = page_begin + (int64_t)it * PG;
+      const int npg = (int)min((int64_t)PG, page_end - first);
+      int64_t blk = next_blk;
+      const int64_t ahead = first + PG + my_page;
+      if (mine && it + 1 < n_iter && ahead < page_end) next_blk = table[ahead];
+      if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], (uint32_t)npg * 2 * kBytes);
+      __syncwarp();
+      if (mine && my_page < npg) {
+        if (blk < 0 || blk >= a.num_blocks) {
+          record_status(MI_STATUS_BAD_BLOCK);
+          blk = 0;  // the null block
+        }
+        bulk_load(smem + st * S::kStageBytes + lane * kBytes, pool + blk * block_bytes, kBytes, &full_bar[st]);
+      }
+    }
+    return;
+  }
+
+  // ---------------- consumers: one warp per (KV head, page of the stage) ----------------
+  const int hl = warp / PG;
+  const int pg = warp % PG;
+  const int h = head0 + hl;
+  const int r = lane >> 2;  // MMA row (token or value) and, of a B operand, its column (query head)
+  const int t = lane & 3;
+
+  // q as the B operand of S^T: this lane holds head r's values d = 32 g + 8 t + 0..7 of every group
+  uint32_t qb[NG][4];
+  float qsum[NG];  // of the whole group
+  float unit;      // what one unit of q * (code operand) stands for, times the softmax scale
+  {
+    float qv[NG][8];
+    const bool valid = r < a.groups;
+    const T* qp = reinterpret_cast<const T*>(a.q + b * a.q_sb + (int64_t)(h * a.groups + (valid ? r : 0)) * a.q_sh);
+    float top = 0.f;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      qsum[g] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        qv[g][i] = valid ? Elem<T>::to_f(qp[g * kKv4Group + t * 8 + i]) : 0.f;
+        top = fmaxf(top, fabsf(qv[g][i]));
+        qsum[g] += qv[g][i];
+      }
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e+1)
+    const float up = pow2(14 - e);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
+      qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
+      qsum[g] *= a.scale_log2;
+      float u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = qv[g][i] * up * ((i & 1) ? 0.0625f : 1.f);
+      qb[g][0] = pack2<__half>(u[0], u[4]);
+      qb[g][1] = pack2<__half>(u[1], u[5]);
+      qb[g][2] = pack2<__half>(u[2], u[6]);
+      qb[g][3] = pack2<__half>(u[3], u[7]);
+    }
+    unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
+  }
+  // An accumulator's columns are heads 2t and 2t + 1: their sums and units, from the lanes that hold them.
+  float qs[2][NG], un[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    un[c] = __shfl_sync(0xffffffffu, unit, (2 * t + c) * 4);
+#pragma unroll
+    for (int g = 0; g < NG; ++g) qs[c][g] = __shfl_sync(0xffffffffu, qsum[g], (2 * t + c) * 4);
+  }
+
+  float o[D / 16][4];  // O^T: rows are values, columns heads 2t, 2t + 1
+  float z[NG][2];      // sum p m of this lane's tokens
+  float l[2] = {0.f, 0.f};
+  float ref[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
+
+  for (int it = 0; it < n_iter; ++it) {
+    const int st = it % NST;
+    mbar_wait(&full_bar[st], (it / NST) & 1, aborted);
+    const int64_t page = page_begin + (int64_t)it * PG + pg;
+    if (page < page_end) {
+      const uint8_t* k_page = smem + st * S::kStageBytes + (pg * 2 * HB + hl) * S::kPageBytes;
+      const uint8_t* v_page = k_page + HB * S::kPageBytes;
+      const int left = (int)min((int64_t)BS, ctx - page * BS);  // tokens of this page
+#pragma unroll 1
+      for (int step = 0; step < BS / 16; ++step) {
+        const int tok0 = step * 16;
+        if (tok0 >= left) break;
+        // rows of the 8x8 matrices: (token octet, 16 bytes of a group) x two groups
+        const uint32_t row = (uint32_t)(tok0 + ((lane >> 3) & 1) * 8 + (lane & 7) + (lane >> 4) * BS) * 16;
+        const uint32_t k_addr = smem_u32(k_page) + row;
+        const uint32_t v_addr = smem_u32(v_page) + row;
+        const uint8_t* k_par = k_page + BS * D / 2 + (tok0 + r) * NG * 4;
+        const uint8_t* v_par = v_page + BS * D / 2 + (tok0 + r) * NG * 4;
+        // ---- scores of 16 tokens: x[0..1] token r, x[2..3] token r + 8; columns heads 2t, 2t + 1 ----
+        uint32_t kw[2][NG];
+        kv4_params<NG>(k_par, kw[0]);
+        kv4_params<NG>(k_par + 8 * NG * 4, kw[1]);
+        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int gp = 0; gp < NG / 2; ++gp) {
+          uint32_t c[4];
+          ldmatrix_x4(k_addr + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int g = gp * 2 + i;
+            uint32_t lo[4], hi[4];
+            kv4_operands(c[2 * i], lo);
+            kv4_operands(c[2 * i + 1], hi);
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
+            const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+            Mma16816<__half>::run(acc, a0, qb[g][0], qb[g][1]);
+            Mma16816<__half>::run(acc, a1, qb[g][2], qb[g][3]);
+            const float s0 = kv4_step(kw[0][g]), s1 = kv4_step(kw[1][g]);
+            const float m0 = kv4_min(kw[0][g]), m1 = kv4_min(kw[1][g]);
+            x[0] = fmaf(acc[0], s0, x[0]);
+            x[1] = fmaf(acc[1], s0, x[1]);
+            x[2] = fmaf(acc[2], s1, x[2]);
+            x[3] = fmaf(acc[3], s1, x[3]);
+            y[0] = fmaf(m0, qs[0][g], y[0]);
+            y[1] = fmaf(m0, qs[1][g], y[1]);
+            y[2] = fmaf(m1, qs[0][g], y[2]);
+            y[3] = fmaf(m1, qs[1][g], y[3]);
+          }
+        }
+        x[0] = fmaf(x[0], un[0], y[0]);
+        x[1] = fmaf(x[1], un[1], y[1]);
+        x[2] = fmaf(x[2], un[0], y[2]);
+        x[3] = fmaf(x[3], un[1], y[3]);
+        uint32_t vw[2][NG];
+        kv4_params<NG>(v_par, vw[0]);
+        kv4_params<NG>(v_par + 8 * NG * 4, vw[1]);
+        if (tok0 + 16 > left) {  // the sequence ends in this tile: nothing past it counts, whatever it holds
+          if (tok0 + r >= left) {
+            x[0] = x[1] = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) vw[0][g] = 0u;
+          }
+          if (tok0 + r + 8 >= left) {
+            x[2] = x[3] = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) vw[1][g] = 0u;
+          }
+        }
+        // widest step of each token (positive bfloat16s order as integers)
+        uint32_t w0 = vw[0][0], w1 = vw[1][0];
+#pragma unroll
+        for (int g = 1; g < NG; ++g) {
+          w0 = __vmaxu2(w0, vw[0][g]);
+          w1 = __vmaxu2(w1, vw[1][g]);
+        }
+        const float wide[2] = {kv4_step(w0), kv4_step(w1)};
+        // ---- weights against the running reference; it moves only when one would leave fp16's range ----
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = exp2f(x[i] - ref[i & 1]);
+        bool fine = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fine = fine && p[i] * wide[i >> 1] <= kKv4Limit && p[i] <= kKv4PLimit;
+        if (__any_sync(0xffffffffu, !fine)) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float want = fmaxf(kv4_reference(x[c], wide[0]), kv4_reference(x[c + 2], wide[1]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
+            want = fmaxf(want, ref[c]);
+            const float base = want == -INFINITY ? 0.f : want;
+            const float alpha = exp2f(ref[c] - base);  // 0 from the initial -inf
+            l[c] *= alpha;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              o[i][c] *= alpha;
+              o[i][c + 2] *= alpha;
+            }
+            p[c] = exp2f(x[c] - base);
+            p[c + 2] = exp2f(x[c + 2] - base);
+            ref[c] = want;
+          }
+        }
+        l[0] += p[0] + p[2];
+        l[1] += p[1] + p[3];
+        // ---- O^T += V^T (p s)^T, z += p m ----
+#pragma unroll
+        for (int gp = 0; gp < NG / 2; ++gp) {
+          uint32_t c[4];
+          ldmatrix_x4_trans(v_addr + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int g = gp * 2 + i;
+            const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
+            const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
+            z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
+            z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
+            const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
+            const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
+            const uint32_t b0 = movmatrix_trans(h0), b1 = movmatrix_trans(h1);
+            uint32_t lo[4], hi[4];
+            kv4_operands(c[2 * i], lo);
+            kv4_operands(c[2 * i + 1], hi);
+            const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
+            const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
+            Mma16816<__half>::run(o[2 * g], a0, b0, b1);
+            Mma16816<__half>::run(o[2 * g + 1], a1, b0, b1);
+            if constexpr (kTwo) {
+              const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+              const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+              const uint32_t d0 = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
+              const uint32_t d1 = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
+              Mma16816<__half>::run(o[2 * g], a0, d0, d1);
+              Mma16816<__half>::run(o[2 * g + 1], a1, d0, d1);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty_bar[st]);
+  }
+
+  // ---- this warp's partial: sums over the lanes that share columns, then rows (heads 2t, 2t + 1) ----
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+#pragma unroll
+    for (int off = 4; off < 32; off <<= 1) {
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], off);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
+    }
+    const int head = 2 * t + c;
+    if (head >= a.groups) continue;
+    const int64_t hq = (int64_t)h * a.groups + head;
+    const int64_t idx = (b * a.hq + hq) * a.max_parts + split * PG + pg;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {  // values d = 32 g + 4 r + 0..3: rows r of tile 2g, r + 8 (times 16), tile 2g + 1
+      const float v[4] = {fmaf(o[2 * g][c], 0x1p24f, z[g][c]), fmaf(o[2 * g][c + 2], 0x1p20f, z[g][c]),
+                          fmaf(o[2 * g + 1][c], 0x1p24f, z[g][c]), fmaf(o[2 * g + 1][c + 2], 0x1p20f, z[g][c])};
+      *reinterpret_cast<float4*>(a.ws_o + idx * D + g * kKv4Group + r * 4) = make_float4(v[0], v[1], v[2], v[3]);
+    }
+    if (r == 0) *reinterpret_cast<float2*>(a.ws_ml + idx * 2) = make_float2(ref[c], l[c]);
+  }
+}
+
+template <typename T, int D, int BS, int HB>
+cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
+  using S = Kv4Shape<D, BS, HB>;
+  auto kern = kv4_decode_split_kernel<T, D, BS, HB>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.max_splits, (unsigned)(a.hkv / HB), (unsigned)a.batch);
+  cfg.blockDim = dim3(kKv4SplitThreads);
+  cfg.dynamicSmemBytes = S::kSmemBytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, a);
+  if (e != cudaSuccess) return e;
+  DecodeArgs d{};
+  d.context_lens = a.context_lens;
+  d.batch = a.batch;
+  d.max_blocks = a.max_blocks;
+  d.hq = a.hq;
+  d.head_dim = D;
+  d.block_size = BS;
+  d.split_pages = a.split_pages;
+  d.parts_per_split = S::kPages;
+  d.max_parts = a.max_parts;
+  d.ws_o = a.ws_o;
+  d.ws_ml = a.ws_ml;
+  d.out = a.out;
+  d.out_sb = a.out_sb;
+  cfg.gridDim = dim3((unsigned)((a.batch * a.hq + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  return cudaLaunchKernelEx(&cfg, decode_combine_kernel<T, D>, d);
+}
+
+template <typename T, int D, int BS>
+cudaError_t launch_kv4_split_hb(const Kv4DecodeArgs& a, int hb, cudaStream_t s) {
+  switch (hb) {
+    case 4: return launch_kv4_split<T, D, BS, 4>(a, s);
+    case 2: return launch_kv4_split<T, D, BS, 2>(a, s);
+    default: return launch_kv4_split<T, D, BS, 1>(a, s);
+  }
+}
+
+template <typename T>
+cudaError_t launch_kv4_split_t(const Kv4DecodeArgs& a, int hb, cudaStream_t s) {
+  if (a.head_dim == 128)
+    return a.block_size == 16 ? launch_kv4_split_hb<T, 128, 16>(a, hb, s) : launch_kv4_split_hb<T, 128, 32>(a, hb, s);
+  return a.block_size == 16 ? launch_kv4_split_hb<T, 64, 16>(a, hb, s) : launch_kv4_split_hb<T, 64, 32>(a, hb, s);
+}
+
 }  // namespace
 
 Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int64_t max_blocks, int block_size,
                               int dtype) {
-  (void)batch, (void)hq, (void)hkv, (void)head_dim, (void)max_blocks, (void)block_size, (void)dtype;
-  return Kv4DecodePlan{};
+  Kv4DecodePlan p{};
+  const int groups = hq / hkv;
+  p.use_mma = (dtype == MI_BF16 || dtype == MI_F16) && (head_dim == 64 || head_dim == 128) &&
+              (block_size == 16 || block_size == 32) && groups >= 1 && groups <= 8;
+  if (!p.use_mma) return p;
+  p.heads_per_cta = (hkv % 4 == 0) ? 4 : (hkv % 2 == 0) ? 2 : 1;
+  p.parts_per_split = kKv4Consumers / p.heads_per_cta;
+  // Splits of 1024 tokens x 4 KV heads per CTA, halved while the grid would not cover the SMs twice.
+  const int64_t ctas = batch * (hkv / p.heads_per_cta);
+  int64_t pages = std::max<int64_t>(p.parts_per_split, 1024 * p.parts_per_split / block_size);
+  while (pages > p.parts_per_split && ctas * ((max_blocks + pages - 1) / pages) < 2 * 148 * 3)
+    pages = std::max<int64_t>(p.parts_per_split, pages / 2);
+  p.split_pages = (int)std::min<int64_t>(pages, max_blocks);
+  p.max_splits = (int)((max_blocks + p.split_pages - 1) / p.split_pages);
+  const size_t rows = (size_t)batch * hq * p.max_splits * p.parts_per_split;
+  p.ws_bytes = ((rows * head_dim * sizeof(float) + 255) & ~size_t(255)) + ((rows * 8 + 255) & ~size_t(255));
+  return p;
 }
 
 cudaError_t launch_kv4_decode(const Kv4DecodeArgs& a, const Kv4DecodePlan& plan, int dtype, cudaStream_t s) {
-  (void)plan;
+  if (plan.use_mma) {
+    if (dtype == MI_BF16) return launch_kv4_split_t<__nv_bfloat16>(a, plan.heads_per_cta, s);
+    return launch_kv4_split_t<__half>(a, plan.heads_per_cta, s);
+  }
   const unsigned grid = (unsigned)(a.batch * a.hq);
   if (dtype == MI_BF16) kv4_decode_generic_kernel<__nv_bfloat16><<<grid, kKv4Warps * 32, 0, s>>>(a);
   else if (dtype == MI_F16) kv4_decode_generic_kernel<__half><<<grid, kKv4Warps * 32, 0, s>>>(a);
