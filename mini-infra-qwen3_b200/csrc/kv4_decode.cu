@@ -16,9 +16,9 @@
 //     because p s differs by group.
 //   * q is scaled by a power of two to a largest value in [2^14, 2^15) and held in fp16: exact for the
 //     16-bit types except far below the row's largest value (absolute error 2^-24 of it).
-//   * p s is held in fp16.  The running reference of the softmax is that of p * s (see kv4_reference):
-//     products lie in fp16's upper range, rounding them costs 2^-12 of a weight; an fp16 model, whose
-//     output has as many bits, carries the rounding's remainder in a second fp16 operand.
+//   * p s is held in fp16.  The softmax's running reference is one of p * s, not of p: it keeps the largest
+//     product in fp16's upper range, so rounding costs 2^-12 of a weight; an fp16 model, whose output has
+//     as many bits, carries the rounding's remainder in a second fp16 operand.
 //   * Scores, sums, the minimum terms and O are fp32.
 // grid = (splits, KV head blocks, batch); a producer warp brings whole pages (all heads of the block in
 // one bulk copy for K and one for V) into a ring of shared-memory stages, 4 consumer warps each take a
@@ -122,28 +122,25 @@ constexpr int kKv4Consumers = 4;  // consumer warps of the tensor-core kernel's 
 constexpr int kKv4SplitThreads = (kKv4Consumers + 1) * 32;
 constexpr int kKv4Smem = 62 * 1024;  // three CTAs per SM
 
+constexpr int kKv4Unit = 32;  // tokens a consumer warp takes at a time: two 16-row tiles
+
 template <int D, int BS, int HB>
 struct Kv4Shape {
   static constexpr int kGroups = D / kKv4Group;
-  static constexpr int kPages = kKv4Consumers / HB;  // pages of a stage: one (KV head, page) per warp
+  static constexpr int kUnits = kKv4Consumers / HB;     // units of a stage: one (KV head, unit) per warp
+  static constexpr int kUnitPages = kKv4Unit / BS;
+  static constexpr int kPages = kUnits * kUnitPages;    // pages of a stage
   static constexpr int kPageBytes = BS * D / 2 + BS * kGroups * 4;
   static constexpr int kStageBytes = kPages * HB * 2 * kPageBytes;
   static constexpr int kStages = std::max(2, std::min(8, kKv4Smem / kStageBytes));
   static constexpr int kSmemBytes = kStages * (kStageBytes + 16) + 128;
 };
 
-constexpr float kKv4TopLog2 = 11.f;    // p * s of a new reference: at most 2^11
-constexpr float kKv4Limit = 32768.f;   // p * s above this moves the reference (fp16 ends at 65504)
-constexpr float kKv4PLog2 = 60.f;      // p alone of a new reference: at most 2^60
-constexpr float kKv4PLimit = 0x1p68f;
+constexpr float kKv4TopLog2 = 11.f;   // p * s of a new reference: at most 2^11
+constexpr float kKv4Limit = 32768.f;  // p * s above this moves the reference (fp16 ends at 65504)
+constexpr float kKv4Narrow = 0x1p-53f;  // steps below this count as this: p stays below 2^68 whatever the steps
 
 __device__ __forceinline__ float pow2(int n) { return __uint_as_float((uint32_t)(n + 127) << 23); }  // -126 <= n <= 128
-
-// The reference a token asks for: weights are exp2(x - reference), x the score in powers of two, so
-// that p * s <= 2^11 for its widest step s, and p <= 2^60 where the steps are (nearly) zero.
-__device__ __forceinline__ float kv4_reference(float x, float widest) {
-  return x + fmaxf(log2f(widest) - kKv4TopLog2, -kKv4PLog2);
-}
 
 // Four operands out of eight codes: codes (0, 4), (1, 5) times 16, (2, 6), (3, 7) times 16, as halves
 // in units of 2^-24.
@@ -172,6 +169,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
   constexpr int NG = S::kGroups;
   constexpr int NST = S::kStages;
   constexpr int PG = S::kPages;
+  constexpr int UN = S::kUnits;
   constexpr bool kTwo = std::is_same<T, __half>::value;  // p * s as two fp16 operands
   asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the append
   extern __shared__ uint8_t smem_raw[];
@@ -240,19 +238,19 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     return;
   }
 
-  // ---------------- consumers: one warp per (KV head, page of the stage) ----------------
-  const int hl = warp / PG;
-  const int pg = warp % PG;
+  // ---------------- consumers: one warp per (KV head, unit of 32 tokens) ----------------
+  const int hl = warp / UN;
+  const int un = warp % UN;
   const int h = head0 + hl;
   const int r = lane >> 2;  // MMA row (token or value) and, of a B operand, its column (query head)
   const int t = lane & 3;
 
   // q as the B operand of S^T: this lane holds head r's values d = 32 g + 8 t + 0..7 of every group
   uint32_t qb[NG][4];
-  float qsum[NG];  // of the whole group
-  float unit;      // what one unit of q * (code operand) stands for, times the softmax scale
+  uint32_t mb[3];  // B operands of the minimum term, see below
+  float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: heads 2t, 2t + 1
   {
-    float qv[NG][8];
+    float qv[NG][8], qsum[NG];
     const bool valid = r < a.groups;
     const T* qp = reinterpret_cast<const T*>(a.q + b * a.q_sb + (int64_t)(h * a.groups + (valid ? r : 0)) * a.q_sh);
     float top = 0.f;
@@ -283,15 +281,27 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
       qb[g][2] = pack2<__half>(u[2], u[6]);
       qb[g][3] = pack2<__half>(u[3], u[7]);
     }
-    unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
-  }
-  // An accumulator's columns are heads 2t and 2t + 1: their sums and units, from the lanes that hold them.
-  float qs[2][NG], un[2];
+    // The minimum term sum_g m_g sum(q_g) as a bf16 MMA on the parameter words themselves: columns 2t
+    // and 2t + 1 of a token's row are (s, m) of group t % NG.  The steps meet zeros; sum(q_g) enters
+    // as three bfloat16s, 24 bits of it: in k 2t + 1, in k 2t + 9 and in a second MMA (NG = 4), or in
+    // k 2t + 1 of both pairs of lanes and in k 2t + 9 (NG = 2).
+    float mine = qsum[0];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    un[c] = __shfl_sync(0xffffffffu, unit, (2 * t + c) * 4);
+    for (int g = 1; g < NG; ++g) mine = (t % NG) == g ? qsum[g] : mine;
+    uint32_t part[3];
 #pragma unroll
-    for (int g = 0; g < NG; ++g) qs[c][g] = __shfl_sync(0xffffffffu, qsum[g], (2 * t + c) * 4);
+    for (int i = 0; i < 3; ++i) {
+      part[i] = bf16_bits(mine);
+      mine -= __uint_as_float(part[i] << 16);
+    }
+    if constexpr (NG == 4) {
+      mb[0] = part[0] << 16, mb[1] = part[1] << 16, mb[2] = part[2] << 16;
+    } else {
+      mb[0] = (t < 2 ? part[0] : part[1]) << 16, mb[1] = t < 2 ? part[2] << 16 : 0u, mb[2] = 0u;
+    }
+    const float mine_unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
+    unit[0] = __shfl_sync(0xffffffffu, mine_unit, 8 * t);  // accumulator columns are heads 2t, 2t + 1
+    unit[1] = __shfl_sync(0xffffffffu, mine_unit, 8 * t + 4);
   }
 
   float o[D / 16][4];  // O^T: rows are values, columns heads 2t, 2t + 1
@@ -303,132 +313,159 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
 #pragma unroll
   for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
 
-  for (int it = 0; it < n_iter; ++it) {
+  // rows of the 8x8 matrices: (token octet, 16 bytes of a group) x two groups
+  const uint32_t mat_row = (uint32_t)(((lane >> 3) & 1) * 8 + (lane & 7) + (lane >> 4) * BS) * 16;
+  constexpr uint32_t kPar = BS * D / 2;  // of a page
+  const uint32_t k_off = (un * S::kUnitPages * 2 * HB + hl) * S::kPageBytes;
+  int left = (int)(min(ctx, page_end * BS) - page_begin * BS) - un * kKv4Unit;  // tokens from this unit on
+
+  for (int it = 0; it < n_iter; ++it, left -= UN * kKv4Unit) {
     const int st = it % NST;
     mbar_wait(&full_bar[st], (it / NST) & 1, aborted);
-    const int64_t page = page_begin + (int64_t)it * PG + pg;
-    if (page < page_end) {
-      const uint8_t* k_page = smem + st * S::kStageBytes + (pg * 2 * HB + hl) * S::kPageBytes;
-      const uint8_t* v_page = k_page + HB * S::kPageBytes;
-      const int left = (int)min((int64_t)BS, ctx - page * BS);  // tokens of this page
-#pragma unroll 1
-      for (int step = 0; step < BS / 16; ++step) {
-        const int tok0 = step * 16;
-        if (tok0 >= left) break;
-        // rows of the 8x8 matrices: (token octet, 16 bytes of a group) x two groups
-        const uint32_t row = (uint32_t)(tok0 + ((lane >> 3) & 1) * 8 + (lane & 7) + (lane >> 4) * BS) * 16;
-        const uint32_t k_addr = smem_u32(k_page) + row;
-        const uint32_t v_addr = smem_u32(v_page) + row;
-        const uint8_t* k_par = k_page + BS * D / 2 + (tok0 + r) * NG * 4;
-        const uint8_t* v_par = v_page + BS * D / 2 + (tok0 + r) * NG * 4;
-        // ---- scores of 16 tokens: x[0..1] token r, x[2..3] token r + 8; columns heads 2t, 2t + 1 ----
+    if (left > 0) {
+      const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
+      // tile i's K page, its token offset in the page; V pages lie HB pages further
+      auto page_of = [&](int i) { return k_unit + (BS == 16 ? i * 2 * HB * S::kPageBytes : 0); };
+      auto tok_of = [&](int i) { return BS == 16 ? 0 : i * 16; };
+      // ---- scores of 2 x 16 tokens: x[i][0..1] token r, [2..3] token r + 8; columns heads 2t, 2t + 1 ----
+      float x[2][4], wide[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* k_page = page_of(i);
+        const uint8_t* k_par = k_page + kPar + (tok_of(i) + r) * NG * 4;
+        const uint32_t mw[4] = {*reinterpret_cast<const uint32_t*>(k_par + (t % NG) * 4),
+                                *reinterpret_cast<const uint32_t*>(k_par + (8 * NG + t % NG) * 4), 0u, 0u};
+        float y[4];
+        const uint32_t mw2[4] = {mw[0], mw[1], mw[0], mw[1]};
+        Mma16816<__nv_bfloat16>::zero(y, mw2, mb[0], mb[1]);
+        if constexpr (NG == 4) Mma16816<__nv_bfloat16>::run(y, mw, mb[2], 0u);
         uint32_t kw[2][NG];
         kv4_params<NG>(k_par, kw[0]);
         kv4_params<NG>(k_par + 8 * NG * 4, kw[1]);
-        float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+        float s[4];
 #pragma unroll
         for (int gp = 0; gp < NG / 2; ++gp) {
           uint32_t c[4];
-          ldmatrix_x4(k_addr + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+          ldmatrix_x4(smem_u32(k_page) + tok_of(i) * 16 + mat_row + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int g = gp * 2 + i;
+          for (int j = 0; j < 2; ++j) {
+            const int g = gp * 2 + j;
             uint32_t lo[4], hi[4];
-            kv4_operands(c[2 * i], lo);
-            kv4_operands(c[2 * i + 1], hi);
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            kv4_operands(c[2 * j], lo);
+            kv4_operands(c[2 * j + 1], hi);
+            float acc[4];
             const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
             const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-            Mma16816<__half>::run(acc, a0, qb[g][0], qb[g][1]);
+            Mma16816<__half>::zero(acc, a0, qb[g][0], qb[g][1]);
             Mma16816<__half>::run(acc, a1, qb[g][2], qb[g][3]);
             const float s0 = kv4_step(kw[0][g]), s1 = kv4_step(kw[1][g]);
-            const float m0 = kv4_min(kw[0][g]), m1 = kv4_min(kw[1][g]);
-            x[0] = fmaf(acc[0], s0, x[0]);
-            x[1] = fmaf(acc[1], s0, x[1]);
-            x[2] = fmaf(acc[2], s1, x[2]);
-            x[3] = fmaf(acc[3], s1, x[3]);
-            y[0] = fmaf(m0, qs[0][g], y[0]);
-            y[1] = fmaf(m0, qs[1][g], y[1]);
-            y[2] = fmaf(m1, qs[0][g], y[2]);
-            y[3] = fmaf(m1, qs[1][g], y[3]);
+            s[0] = g ? fmaf(acc[0], s0, s[0]) : acc[0] * s0;
+            s[1] = g ? fmaf(acc[1], s0, s[1]) : acc[1] * s0;
+            s[2] = g ? fmaf(acc[2], s1, s[2]) : acc[2] * s1;
+            s[3] = g ? fmaf(acc[3], s1, s[3]) : acc[3] * s1;
           }
         }
-        x[0] = fmaf(x[0], un[0], y[0]);
-        x[1] = fmaf(x[1], un[1], y[1]);
-        x[2] = fmaf(x[2], un[0], y[2]);
-        x[3] = fmaf(x[3], un[1], y[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[i][j] = fmaf(s[j], unit[j & 1], y[j]);
+        // widest step of each token (positive bfloat16s order as integers)
+        const uint8_t* v_par = k_par + HB * S::kPageBytes;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t vw[NG];
+          kv4_params<NG>(v_par + j * 8 * NG * 4, vw);
+          uint32_t w = vw[0];
+#pragma unroll
+          for (int g = 1; g < NG; ++g) w = __vmaxu2(w, vw[g]);
+          wide[i][j] = fmaxf(kv4_step(w), kKv4Narrow);
+        }
+      }
+      const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
+      if (tail) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (i * 16 + j * 8 + r >= left) {
+              x[i][2 * j] = x[i][2 * j + 1] = -INFINITY;
+              wide[i][j] = kKv4Narrow;
+            }
+      }
+      // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
+      // then to where the largest p * s of this unit is 2^11 ----
+      float p[2][4];
+      float most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[i][j] = ex2_approx(x[i][j] - ref[j & 1]);
+        most = fmaxf(most, fmaxf(fmaxf(p[i][0], p[i][1]) * wide[i][0], fmaxf(p[i][2], p[i][3]) * wide[i][1]));
+      }
+      if (__any_sync(0xffffffffu, most > kKv4Limit)) {
+        float wl[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) wl[i][j] = log2f(wide[i][j]) - kKv4TopLog2;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float want = fmaxf(fmaxf(x[0][c] + wl[0][0], x[0][c + 2] + wl[0][1]),
+                             fmaxf(x[1][c] + wl[1][0], x[1][c + 2] + wl[1][1]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
+          want = fmaxf(want, ref[c]);
+          const float base = want == -INFINITY ? 0.f : want;
+          const float alpha = ex2_approx(ref[c] - base);  // 0 from the initial -inf
+          l[c] *= alpha;
+#pragma unroll
+          for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            o[i][c] *= alpha;
+            o[i][c + 2] *= alpha;
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            p[i][c] = ex2_approx(x[i][c] - base);
+            p[i][c + 2] = ex2_approx(x[i][c + 2] - base);
+          }
+          ref[c] = want;
+        }
+      }
+      // ---- O^T += V^T (p s)^T, z += p m ----
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* v_page = page_of(i) + HB * S::kPageBytes;
+        const uint8_t* v_par = v_page + kPar + (tok_of(i) + r) * NG * 4;
+        l[0] += p[i][0] + p[i][2];
+        l[1] += p[i][1] + p[i][3];
         uint32_t vw[2][NG];
         kv4_params<NG>(v_par, vw[0]);
         kv4_params<NG>(v_par + 8 * NG * 4, vw[1]);
-        if (tok0 + 16 > left) {  // the sequence ends in this tile: nothing past it counts, whatever it holds
-          if (tok0 + r >= left) {
-            x[0] = x[1] = -INFINITY;
+        if (tail) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) vw[0][g] = 0u;
-          }
-          if (tok0 + r + 8 >= left) {
-            x[2] = x[3] = -INFINITY;
+          for (int j = 0; j < 2; ++j)
+            if (i * 16 + j * 8 + r >= left) {
 #pragma unroll
-            for (int g = 0; g < NG; ++g) vw[1][g] = 0u;
-          }
-        }
-        // widest step of each token (positive bfloat16s order as integers)
-        uint32_t w0 = vw[0][0], w1 = vw[1][0];
-#pragma unroll
-        for (int g = 1; g < NG; ++g) {
-          w0 = __vmaxu2(w0, vw[0][g]);
-          w1 = __vmaxu2(w1, vw[1][g]);
-        }
-        const float wide[2] = {kv4_step(w0), kv4_step(w1)};
-        // ---- weights against the running reference; it moves only when one would leave fp16's range ----
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = exp2f(x[i] - ref[i & 1]);
-        bool fine = true;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) fine = fine && p[i] * wide[i >> 1] <= kKv4Limit && p[i] <= kKv4PLimit;
-        if (__any_sync(0xffffffffu, !fine)) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float want = fmaxf(kv4_reference(x[c], wide[0]), kv4_reference(x[c + 2], wide[1]));
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
-            want = fmaxf(want, ref[c]);
-            const float base = want == -INFINITY ? 0.f : want;
-            const float alpha = exp2f(ref[c] - base);  // 0 from the initial -inf
-            l[c] *= alpha;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              o[i][c] *= alpha;
-              o[i][c + 2] *= alpha;
+              for (int g = 0; g < NG; ++g) vw[j][g] = 0u;
             }
-            p[c] = exp2f(x[c] - base);
-            p[c + 2] = exp2f(x[c + 2] - base);
-            ref[c] = want;
-          }
         }
-        l[0] += p[0] + p[2];
-        l[1] += p[1] + p[3];
-        // ---- O^T += V^T (p s)^T, z += p m ----
 #pragma unroll
         for (int gp = 0; gp < NG / 2; ++gp) {
           uint32_t c[4];
-          ldmatrix_x4_trans(v_addr + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+          ldmatrix_x4_trans(smem_u32(v_page) + tok_of(i) * 16 + mat_row + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int g = gp * 2 + i;
+          for (int j = 0; j < 2; ++j) {
+            const int g = gp * 2 + j;
             const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
             const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
-            z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
-            z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
-            const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
+            z[g][0] = fmaf(p[i][2], m1, fmaf(p[i][0], m0, z[g][0]));
+            z[g][1] = fmaf(p[i][3], m1, fmaf(p[i][1], m0, z[g][1]));
+            const float f[4] = {p[i][0] * s0, p[i][1] * s0, p[i][2] * s1, p[i][3] * s1};
             const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
             const uint32_t b0 = movmatrix_trans(h0), b1 = movmatrix_trans(h1);
             uint32_t lo[4], hi[4];
-            kv4_operands(c[2 * i], lo);
-            kv4_operands(c[2 * i + 1], hi);
+            kv4_operands(c[2 * j], lo);
+            kv4_operands(c[2 * j + 1], hi);
             const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
             const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
             Mma16816<__half>::run(o[2 * g], a0, b0, b1);
@@ -461,7 +498,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     const int head = 2 * t + c;
     if (head >= a.groups) continue;
     const int64_t hq = (int64_t)h * a.groups + head;
-    const int64_t idx = (b * a.hq + hq) * a.max_parts + split * PG + pg;
+    const int64_t idx = (b * a.hq + hq) * a.max_parts + split * UN + un;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {  // values d = 32 g + 4 r + 0..3: rows r of tile 2g, r + 8 (times 16), tile 2g + 1
       const float v[4] = {fmaf(o[2 * g][c], 0x1p24f, z[g][c]), fmaf(o[2 * g][c + 2], 0x1p20f, z[g][c]),
@@ -498,7 +535,7 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
   d.head_dim = D;
   d.block_size = BS;
   d.split_pages = a.split_pages;
-  d.parts_per_split = S::kPages;
+  d.parts_per_split = S::kUnits;
   d.max_parts = a.max_parts;
   d.ws_o = a.ws_o;
   d.ws_ml = a.ws_ml;
@@ -537,12 +574,13 @@ Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int6
   if (!p.use_mma) return p;
   p.heads_per_cta = (hkv % 4 == 0) ? 4 : (hkv % 2 == 0) ? 2 : 1;
   p.parts_per_split = kKv4Consumers / p.heads_per_cta;
-  // Splits of 1024 tokens x 4 KV heads per CTA, halved while the grid would not cover the SMs twice.
+  // Splits of 1024 tokens x 4 KV heads per CTA, halved while the grid would not cover the SMs twice; at
+  // least one unit a warp.
   const int64_t ctas = batch * (hkv / p.heads_per_cta);
-  int64_t pages = std::max<int64_t>(p.parts_per_split, 1024 * p.parts_per_split / block_size);
-  while (pages > p.parts_per_split && ctas * ((max_blocks + pages - 1) / pages) < 2 * 148 * 3)
-    pages = std::max<int64_t>(p.parts_per_split, pages / 2);
-  p.split_pages = (int)std::min<int64_t>(pages, max_blocks);
+  const int64_t least = p.parts_per_split * (kKv4Unit / block_size);
+  int64_t pages = 1024 * p.parts_per_split / block_size;
+  while (pages > least && ctas * ((max_blocks + pages - 1) / pages) < 2 * 148 * 3) pages /= 2;
+  p.split_pages = (int)pages;
   p.max_splits = (int)((max_blocks + p.split_pages - 1) / p.split_pages);
   const size_t rows = (size_t)batch * hq * p.max_splits * p.parts_per_split;
   p.ws_bytes = ((rows * head_dim * sizeof(float) + 255) & ~size_t(255)) + ((rows * 8 + 255) & ~size_t(255));
