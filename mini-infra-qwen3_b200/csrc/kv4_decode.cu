@@ -163,7 +163,7 @@ __device__ __forceinline__ void kv4_params(const uint8_t* p, uint32_t (&w)[NG]) 
   }
 }
 
-template <typename T, int D, int BS, int HB>
+template <typename T, int D, int BS, int HB, int SH>
 __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(const Kv4DecodeArgs a) {
   using S = Kv4Shape<D, BS, HB>;
   constexpr int NG = S::kGroups;
@@ -245,14 +245,18 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
   const int r = lane >> 2;  // MMA row (token or value) and, of a B operand, its column (query head)
   const int t = lane & 3;
 
-  // q as the B operand of S^T: this lane holds head r's values d = 32 g + 8 t + 0..7 of every group
+  // q as the B operand of S^T: this lane holds column r's values d = 32 g + 8 t + 0..7 of every group.
+  // Column c is query head c % kCols; with SH = 2 the first four columns are for the first tile's
+  // tokens, the last four for the second's.
+  constexpr int kCols = 8 / SH;
   uint32_t qb[NG][4];
   uint32_t mb[3];  // B operands of the minimum term, see below
-  float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: heads 2t, 2t + 1
+  float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: columns 2t, 2t + 1
   {
     float qv[NG][8], qsum[NG];
-    const bool valid = r < a.groups;
-    const T* qp = reinterpret_cast<const T*>(a.q + b * a.q_sb + (int64_t)(h * a.groups + (valid ? r : 0)) * a.q_sh);
+    const bool valid = r % kCols < a.groups;
+    const T* qp =
+        reinterpret_cast<const T*>(a.q + b * a.q_sb + (int64_t)(h * a.groups + (valid ? r % kCols : 0)) * a.q_sh);
     float top = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -300,11 +304,11 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
       mb[0] = (t < 2 ? part[0] : part[1]) << 16, mb[1] = t < 2 ? part[2] << 16 : 0u, mb[2] = 0u;
     }
     const float mine_unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
-    unit[0] = __shfl_sync(0xffffffffu, mine_unit, 8 * t);  // accumulator columns are heads 2t, 2t + 1
+    unit[0] = __shfl_sync(0xffffffffu, mine_unit, 8 * t);  // accumulator columns 2t, 2t + 1
     unit[1] = __shfl_sync(0xffffffffu, mine_unit, 8 * t + 4);
   }
 
-  float o[D / 16][4];  // O^T: rows are values, columns heads 2t, 2t + 1
+  float o[D / 16][4];  // O^T: rows are values, columns 2t, 2t + 1
   float z[NG][2];      // sum p m of this lane's tokens
   float l[2] = {0.f, 0.f};
   float ref[2] = {-INFINITY, -INFINITY};
@@ -319,97 +323,116 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
   const uint32_t k_off = (un * S::kUnitPages * 2 * HB + hl) * S::kPageBytes;
   int left = (int)(min(ctx, page_end * BS) - page_begin * BS) - un * kKv4Unit;  // tokens from this unit on
 
+  // The unit's two tiles: tile i's K page and the token offset in it (V pages lie HB pages further); and
+  // the tile of this lane's weights, which are one set of four for both tiles (SH = 2) or one for each.
+  constexpr int kSets = 2 / SH;
+  constexpr int kTilePage = BS == 16 ? 2 * HB * S::kPageBytes : 0;
+  constexpr int kTileTok = BS == 16 ? 0 : 16;
+  const int my_tile = SH == 2 ? t >> 1 : 0;
+  const uint32_t my_par = my_tile * (kTilePage + kTileTok * NG * 4) + kPar + r * NG * 4;
+  const uint32_t col_mask = r < 4 ? 0xffffffffu : 0u;  // SH = 2: the columns of the first tile
+
   for (int it = 0; it < n_iter; ++it, left -= UN * kKv4Unit) {
     const int st = it % NST;
     mbar_wait(&full_bar[st], (it / NST) & 1, aborted);
     if (left > 0) {
       const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
-      // tile i's K page, its token offset in the page; V pages lie HB pages further
-      auto page_of = [&](int i) { return k_unit + (BS == 16 ? i * 2 * HB * S::kPageBytes : 0); };
-      auto tok_of = [&](int i) { return BS == 16 ? 0 : i * 16; };
-      // ---- scores of 2 x 16 tokens: x[i][0..1] token r, [2..3] token r + 8; columns heads 2t, 2t + 1 ----
-      float x[2][4], wide[2][2];
+      const uint32_t k_mat = smem_u32(k_unit) + mat_row;
+      const uint32_t v_mat = k_mat + HB * S::kPageBytes;
+      const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
+      // ---- scores: x[n][0..1] token r, [2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
+      float x[kSets][4], wide[kSets][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint8_t* k_page = page_of(i);
-        const uint8_t* k_par = k_page + kPar + (tok_of(i) + r) * NG * 4;
-        const uint32_t mw[4] = {*reinterpret_cast<const uint32_t*>(k_par + (t % NG) * 4),
-                                *reinterpret_cast<const uint32_t*>(k_par + (8 * NG + t % NG) * 4), 0u, 0u};
-        float y[4];
-        const uint32_t mw2[4] = {mw[0], mw[1], mw[0], mw[1]};
-        Mma16816<__nv_bfloat16>::zero(y, mw2, mb[0], mb[1]);
-        if constexpr (NG == 4) Mma16816<__nv_bfloat16>::run(y, mw, mb[2], 0u);
+      for (int n = 0; n < kSets; ++n) {
+        const uint8_t* k_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4);
         uint32_t kw[2][NG];
         kv4_params<NG>(k_par, kw[0]);
         kv4_params<NG>(k_par + 8 * NG * 4, kw[1]);
-        float s[4];
+        float y[4], s[4];
+#pragma unroll
+        for (int i = 0; i < SH; ++i) {  // the minimum term
+          const uint8_t* par = k_unit + (n + i) * (kTilePage + kTileTok * NG * 4) + kPar + (r * NG + t % NG) * 4;
+          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(par);
+          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4);
+          const uint32_t both[4] = {w0, w1, w0, w1}, once[4] = {w0, w1, 0u, 0u};
+          float u[4];
+          Mma16816<__nv_bfloat16>::zero(u, both, mb[0], mb[1]);
+          if constexpr (NG == 4) Mma16816<__nv_bfloat16>::run(u, once, mb[2], 0u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = i && my_tile == 0 ? y[j] : u[j];
+        }
 #pragma unroll
         for (int gp = 0; gp < NG / 2; ++gp) {
-          uint32_t c[4];
-          ldmatrix_x4(smem_u32(k_page) + tok_of(i) * 16 + mat_row + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+          float acc[2][4];
+#pragma unroll
+          for (int i = 0; i < SH; ++i) {
+            uint32_t c[4];
+            ldmatrix_x4(k_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t lo[4], hi[4];
+              kv4_operands(c[2 * j], lo);
+              kv4_operands(c[2 * j + 1], hi);
+              const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
+              const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+              float u[4];
+              Mma16816<__half>::zero(u, a0, qb[gp * 2 + j][0], qb[gp * 2 + j][1]);
+              Mma16816<__half>::run(u, a1, qb[gp * 2 + j][2], qb[gp * 2 + j][3]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[j][e] = i && my_tile == 0 ? acc[j][e] : u[e];
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int g = gp * 2 + j;
-            uint32_t lo[4], hi[4];
-            kv4_operands(c[2 * j], lo);
-            kv4_operands(c[2 * j + 1], hi);
-            float acc[4];
-            const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
-            const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-            Mma16816<__half>::zero(acc, a0, qb[g][0], qb[g][1]);
-            Mma16816<__half>::run(acc, a1, qb[g][2], qb[g][3]);
             const float s0 = kv4_step(kw[0][g]), s1 = kv4_step(kw[1][g]);
-            s[0] = g ? fmaf(acc[0], s0, s[0]) : acc[0] * s0;
-            s[1] = g ? fmaf(acc[1], s0, s[1]) : acc[1] * s0;
-            s[2] = g ? fmaf(acc[2], s1, s[2]) : acc[2] * s1;
-            s[3] = g ? fmaf(acc[3], s1, s[3]) : acc[3] * s1;
+            s[0] = g ? fmaf(acc[j][0], s0, s[0]) : acc[j][0] * s0;
+            s[1] = g ? fmaf(acc[j][1], s0, s[1]) : acc[j][1] * s0;
+            s[2] = g ? fmaf(acc[j][2], s1, s[2]) : acc[j][2] * s1;
+            s[3] = g ? fmaf(acc[j][3], s1, s[3]) : acc[j][3] * s1;
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[i][j] = fmaf(s[j], unit[j & 1], y[j]);
+        for (int j = 0; j < 4; ++j) x[n][j] = fmaf(s[j], unit[j & 1], y[j]);
         // widest step of each token (positive bfloat16s order as integers)
-        const uint8_t* v_par = k_par + HB * S::kPageBytes;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t vw[NG];
-          kv4_params<NG>(v_par + j * 8 * NG * 4, vw);
+          kv4_params<NG>(k_par + HB * S::kPageBytes + j * 8 * NG * 4, vw);
           uint32_t w = vw[0];
 #pragma unroll
           for (int g = 1; g < NG; ++g) w = __vmaxu2(w, vw[g]);
-          wide[i][j] = fmaxf(kv4_step(w), kKv4Narrow);
+          wide[n][j] = fmaxf(kv4_step(w), kKv4Narrow);
         }
-      }
-      const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
-      if (tail) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
+        if (tail) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (i * 16 + j * 8 + r >= left) {
-              x[i][2 * j] = x[i][2 * j + 1] = -INFINITY;
-              wide[i][j] = kKv4Narrow;
+            if ((n + my_tile) * 16 + j * 8 + r >= left) {
+              x[n][2 * j] = x[n][2 * j + 1] = -INFINITY;
+              wide[n][j] = kKv4Narrow;
             }
+        }
       }
       // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
       // then to where the largest p * s of this unit is 2^11 ----
-      float p[2][4];
+      float p[kSets][4];
       float most = 0.f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int n = 0; n < kSets; ++n) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[i][j] = ex2_approx(x[i][j] - ref[j & 1]);
-        most = fmaxf(most, fmaxf(fmaxf(p[i][0], p[i][1]) * wide[i][0], fmaxf(p[i][2], p[i][3]) * wide[i][1]));
+        for (int j = 0; j < 4; ++j) p[n][j] = ex2_approx(x[n][j] - ref[j & 1]);
+        most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]) * wide[n][0], fmaxf(p[n][2], p[n][3]) * wide[n][1]));
       }
       if (__any_sync(0xffffffffu, most > kKv4Limit)) {
-        float wl[2][2];
+        float ask[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int n = 0; n < kSets; ++n)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) wl[i][j] = log2f(wide[i][j]) - kKv4TopLog2;
+          for (int j = 0; j < 4; ++j)
+            ask[j & 1] = fmaxf(ask[j & 1], x[n][j] + (log2f(wide[n][j >> 1]) - kKv4TopLog2));
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float want = fmaxf(fmaxf(x[0][c] + wl[0][0], x[0][c + 2] + wl[0][1]),
-                             fmaxf(x[1][c] + wl[1][0], x[1][c + 2] + wl[1][1]));
+          float want = ask[c];
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
           want = fmaxf(want, ref[c]);
@@ -424,59 +447,70 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
             o[i][c + 2] *= alpha;
           }
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            p[i][c] = ex2_approx(x[i][c] - base);
-            p[i][c + 2] = ex2_approx(x[i][c + 2] - base);
+          for (int n = 0; n < kSets; ++n) {
+            p[n][c] = ex2_approx(x[n][c] - base);
+            p[n][c + 2] = ex2_approx(x[n][c + 2] - base);
           }
           ref[c] = want;
         }
       }
       // ---- O^T += V^T (p s)^T, z += p m ----
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint8_t* v_page = page_of(i) + HB * S::kPageBytes;
-        const uint8_t* v_par = v_page + kPar + (tok_of(i) + r) * NG * 4;
-        l[0] += p[i][0] + p[i][2];
-        l[1] += p[i][1] + p[i][3];
+      for (int n = 0; n < kSets; ++n) {
+        l[0] += p[n][0] + p[n][2];
+        l[1] += p[n][1] + p[n][3];
+        const uint8_t* v_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4) + HB * S::kPageBytes;
         uint32_t vw[2][NG];
         kv4_params<NG>(v_par, vw[0]);
         kv4_params<NG>(v_par + 8 * NG * 4, vw[1]);
         if (tail) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (i * 16 + j * 8 + r >= left) {
+            if ((n + my_tile) * 16 + j * 8 + r >= left) {
 #pragma unroll
               for (int g = 0; g < NG; ++g) vw[j][g] = 0u;
             }
         }
 #pragma unroll
         for (int gp = 0; gp < NG / 2; ++gp) {
-          uint32_t c[4];
-          ldmatrix_x4_trans(smem_u32(v_page) + tok_of(i) * 16 + mat_row + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+          uint32_t pb[2][kTwo ? 4 : 2];  // p s of the two groups as B operands (and what fp16 left of it)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int g = gp * 2 + j;
             const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
             const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
-            z[g][0] = fmaf(p[i][2], m1, fmaf(p[i][0], m0, z[g][0]));
-            z[g][1] = fmaf(p[i][3], m1, fmaf(p[i][1], m0, z[g][1]));
-            const float f[4] = {p[i][0] * s0, p[i][1] * s0, p[i][2] * s1, p[i][3] * s1};
+            z[g][0] = fmaf(p[n][2], m1, fmaf(p[n][0], m0, z[g][0]));
+            z[g][1] = fmaf(p[n][3], m1, fmaf(p[n][1], m0, z[g][1]));
+            const float f[4] = {p[n][0] * s0, p[n][1] * s0, p[n][2] * s1, p[n][3] * s1};
             const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
-            const uint32_t b0 = movmatrix_trans(h0), b1 = movmatrix_trans(h1);
-            uint32_t lo[4], hi[4];
-            kv4_operands(c[2 * j], lo);
-            kv4_operands(c[2 * j + 1], hi);
-            const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
-            const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
-            Mma16816<__half>::run(o[2 * g], a0, b0, b1);
-            Mma16816<__half>::run(o[2 * g + 1], a1, b0, b1);
+            pb[j][0] = movmatrix_trans(h0);
+            pb[j][1] = movmatrix_trans(h1);
             if constexpr (kTwo) {
               const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
               const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-              const uint32_t d0 = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
-              const uint32_t d1 = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
-              Mma16816<__half>::run(o[2 * g], a0, d0, d1);
-              Mma16816<__half>::run(o[2 * g + 1], a1, d0, d1);
+              pb[j][2] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
+              pb[j][3] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < SH; ++i) {
+            uint32_t c[4];
+            ldmatrix_x4_trans(v_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+            const uint32_t mask = SH == 1 ? 0xffffffffu : i ? ~col_mask : col_mask;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int g = gp * 2 + j;
+              uint32_t lo[4], hi[4];
+              kv4_operands(c[2 * j], lo);
+              kv4_operands(c[2 * j + 1], hi);
+              const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
+              const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
+              Mma16816<__half>::run(o[2 * g], a0, pb[j][0] & mask, pb[j][1] & mask);
+              Mma16816<__half>::run(o[2 * g + 1], a1, pb[j][0] & mask, pb[j][1] & mask);
+              if constexpr (kTwo) {
+                Mma16816<__half>::run(o[2 * g], a0, pb[j][2] & mask, pb[j][3] & mask);
+                Mma16816<__half>::run(o[2 * g + 1], a1, pb[j][2] & mask, pb[j][3] & mask);
+              }
             }
           }
         }
@@ -486,6 +520,30 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     if (lane == 0) mbar_arrive(&empty_bar[st]);
   }
 
+  if constexpr (SH == 2) {
+    // a head's sums over the first and the second tiles meet: columns 2t and 2t + 4
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float other = __shfl_xor_sync(0xffffffffu, ref[c], 2);
+      const float both = fmaxf(ref[c], other);
+      const float alpha = both == -INFINITY ? 1.f : ex2_approx(ref[c] - both);
+      ref[c] = both;
+      l[c] *= alpha;
+      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 2);
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        z[g][c] *= alpha;
+        z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], 2);
+      }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        o[i][c] *= alpha;
+        o[i][c] += __shfl_xor_sync(0xffffffffu, o[i][c], 2);
+        o[i][c + 2] *= alpha;
+        o[i][c + 2] += __shfl_xor_sync(0xffffffffu, o[i][c + 2], 2);
+      }
+    }
+  }
   // ---- this warp's partial: sums over the lanes that share columns, then rows (heads 2t, 2t + 1) ----
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -496,7 +554,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
       for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
     }
     const int head = 2 * t + c;
-    if (head >= a.groups) continue;
+    if (head >= kCols || head >= a.groups) continue;
     const int64_t hq = (int64_t)h * a.groups + head;
     const int64_t idx = (b * a.hq + hq) * a.max_parts + split * UN + un;
 #pragma unroll
@@ -509,10 +567,10 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
   }
 }
 
-template <typename T, int D, int BS, int HB>
+template <typename T, int D, int BS, int HB, int SH>
 cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
   using S = Kv4Shape<D, BS, HB>;
-  auto kern = kv4_decode_split_kernel<T, D, BS, HB>;
+  auto kern = kv4_decode_split_kernel<T, D, BS, HB, SH>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[1];
@@ -550,9 +608,9 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
 template <typename T, int D, int BS>
 cudaError_t launch_kv4_split_hb(const Kv4DecodeArgs& a, int hb, cudaStream_t s) {
   switch (hb) {
-    case 4: return launch_kv4_split<T, D, BS, 4>(a, s);
-    case 2: return launch_kv4_split<T, D, BS, 2>(a, s);
-    default: return launch_kv4_split<T, D, BS, 1>(a, s);
+    case 4: return a.groups <= 4 ? launch_kv4_split<T, D, BS, 4, 2>(a, s) : launch_kv4_split<T, D, BS, 4, 1>(a, s);
+    case 2: return a.groups <= 4 ? launch_kv4_split<T, D, BS, 2, 2>(a, s) : launch_kv4_split<T, D, BS, 2, 1>(a, s);
+    default: return a.groups <= 4 ? launch_kv4_split<T, D, BS, 1, 2>(a, s) : launch_kv4_split<T, D, BS, 1, 1>(a, s);
   }
 }
 
