@@ -213,9 +213,8 @@ int mi_kv4_paged_decode(const void* q, const int64_t* q_strides, const void* k_n
   a.out_sb = out_stride * es;
   a.split_pages = plan.split_pages;
   a.max_splits = plan.max_splits;
-  a.max_parts = plan.max_splits * plan.parts_per_split;
   if (plan.ws_bytes) {
-    const size_t o_bytes = (size_t)batch * num_q_heads * a.max_parts * head_dim * sizeof(float);
+    const size_t o_bytes = (size_t)batch * num_q_heads * a.max_splits * head_dim * sizeof(float);
     a.ws_o = static_cast<float*>(workspace);
     a.ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((o_bytes + 255) & ~size_t(255)));
   }

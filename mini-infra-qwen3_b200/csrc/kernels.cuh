@@ -285,15 +285,13 @@ struct Kv4DecodeArgs {
   int64_t out_sb;  // bytes
   // tensor-core path
   int split_pages;  // pages handled by one split
-  int max_splits;   // grid.x
-  int max_parts;    // partials of one row: max_splits * parts_per_split
-  float* ws_o;      // [batch, hq, max_parts, head_dim]
-  float* ws_ml;     // [batch, hq, max_parts, 2]
+  int max_splits;   // grid.x; 1: the split kernel writes the rows
+  float* ws_o;      // [batch, hq, max_splits, head_dim] partial sums
+  float* ws_ml;     // [batch, hq, max_splits, 2] their references and sums of weights
 };
 struct Kv4DecodePlan {
   bool use_mma;
   int heads_per_cta;
-  int parts_per_split;
   int split_pages;
   int max_splits;
   size_t ws_bytes;

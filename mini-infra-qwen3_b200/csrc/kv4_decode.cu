@@ -22,7 +22,8 @@
 //   * Scores, sums, the minimum terms and O are fp32.
 // grid = (splits, KV head blocks, batch); a producer warp brings whole pages (all heads of the block in
 // one bulk copy for K and one for V) into a ring of shared-memory stages, 4 consumer warps each take a
-// (KV head, page) of a stage.  The splits' partials are merged by decode_combine_kernel.
+// (KV head, 32 tokens) of a stage.  Warps of one KV head merge in shared memory, splits in a second kernel
+// (none where every row is one split).
 //
 // Generic kernel (any type, head_dim, block size and group count): one CTA per (sequence, query head);
 // its warps take the pages in turn, a lane holding value lane of every group, with an online softmax in
@@ -163,6 +164,23 @@ __device__ __forceinline__ void kv4_params(const uint8_t* p, uint32_t (&w)[NG]) 
   }
 }
 
+// Four values of a row's sum, relative to ref, with the sum l of its weights: the output where the row has
+// one split, else the split's partial.
+template <typename T, int D>
+__device__ __forceinline__ void kv4_emit(const Kv4DecodeArgs& a, int64_t b, int hq, int split, int d, const float (&v)[4],
+                                         float ref, float l, bool first) {
+  if (a.max_splits == 1) {
+    T* dst = reinterpret_cast<T*>(a.out + b * a.out_sb) + (int64_t)hq * D + d;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = Elem<T>::from_f(v[i] * inv);
+    return;
+  }
+  const int64_t idx = (b * a.hq + hq) * a.max_splits + split;
+  *reinterpret_cast<float4*>(a.ws_o + idx * D + d) = make_float4(v[0], v[1], v[2], v[3]);
+  if (first) *reinterpret_cast<float2*>(a.ws_ml + idx * 2) = make_float2(ref, l);
+}
+
 template <typename T, int D, int BS, int HB, int SH>
 __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(const Kv4DecodeArgs a) {
   using S = Kv4Shape<D, BS, HB>;
@@ -188,7 +206,12 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     ctx = n_pages * BS;
   }
   const int64_t page_begin = (int64_t)split * a.split_pages;
-  if (page_begin >= n_pages) return;  // uniform for the CTA
+  if (page_begin >= n_pages) {  // uniform for the CTA
+    if (a.max_splits == 1)  // a row of no tokens that no combine follows
+      for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4SplitThreads)
+        reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
+    return;
+  }
   const int64_t page_end = min(n_pages, page_begin + (int64_t)a.split_pages);
   const int n_iter = (int)((page_end - page_begin + PG - 1) / PG);
 
@@ -544,7 +567,8 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
       }
     }
   }
-  // ---- this warp's partial: sums over the lanes that share columns, then rows (heads 2t, 2t + 1) ----
+  // ---- this warp's sums over the lanes that share columns, then its rows: heads 2t, 2t + 1, values
+  // d = 32 g + 4 r + 0..3 (rows r of tile 2g, r + 8 of it, times 16, and of tile 2g + 1) ----
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -553,18 +577,109 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
 #pragma unroll
       for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
     }
-    const int head = 2 * t + c;
-    if (head >= kCols || head >= a.groups) continue;
-    const int64_t hq = (int64_t)h * a.groups + head;
-    const int64_t idx = (b * a.hq + hq) * a.max_parts + split * UN + un;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {  // values d = 32 g + 4 r + 0..3: rows r of tile 2g, r + 8 (times 16), tile 2g + 1
-      const float v[4] = {fmaf(o[2 * g][c], 0x1p24f, z[g][c]), fmaf(o[2 * g][c + 2], 0x1p20f, z[g][c]),
-                          fmaf(o[2 * g + 1][c], 0x1p24f, z[g][c]), fmaf(o[2 * g + 1][c + 2], 0x1p20f, z[g][c])};
-      *reinterpret_cast<float4*>(a.ws_o + idx * D + g * kKv4Group + r * 4) = make_float4(v[0], v[1], v[2], v[3]);
-    }
-    if (r == 0) *reinterpret_cast<float2*>(a.ws_ml + idx * 2) = make_float2(ref[c], l[c]);
   }
+  auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
+  if constexpr (UN > 1) {
+    // The warps of a KV head merge in shared memory; every stage has been consumed.
+    float* so = reinterpret_cast<float*>(smem);                    // [warp][column][D]
+    float* sml = so + kKv4Consumers * kCols * D;                   // [warp][column](ref, l)
+    static_assert((kKv4Consumers * kCols * (D + 2)) * 4 <= NST * S::kStageBytes, "the merge fits the ring");
+    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int col = warp * kCols + 2 * t + c;
+      if (2 * t + c >= kCols) continue;
+#pragma unroll
+      for (int g = 0; g < NG; ++g)
+        *reinterpret_cast<float4*>(so + col * D + g * kKv4Group + r * 4) =
+            make_float4(value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3));
+      if (r == 0) *reinterpret_cast<float2*>(sml + 2 * col) = make_float2(ref[c], l[c]);
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");
+    // four values of one (KV head, query head) at a time
+    constexpr int kVec = D / 4;
+    for (int i = threadIdx.x; i < HB * a.groups * kVec; i += kKv4Consumers * 32) {
+      const int row = i / kVec, d = (i - row * kVec) * 4;
+      const int hm = row / a.groups, head = row - hm * a.groups;
+      float m_all = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < UN; ++u) m_all = fmaxf(m_all, sml[2 * ((hm * UN + u) * kCols + head)]);
+      float l_all = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int col = (hm * UN + u) * kCols + head;
+        const float f = m_all == -INFINITY ? 1.f : ex2_approx(sml[2 * col] - m_all);
+        l_all = fmaf(f, sml[2 * col + 1], l_all);
+        const float4 w = *reinterpret_cast<const float4*>(so + col * D + d);
+        v[0] = fmaf(f, w.x, v[0]), v[1] = fmaf(f, w.y, v[1]), v[2] = fmaf(f, w.z, v[2]), v[3] = fmaf(f, w.w, v[3]);
+      }
+      kv4_emit<T, D>(a, b, (head0 + hm) * a.groups + head, split, d, v, m_all, l_all, d == 0);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int head = 2 * t + c;
+      if (head >= kCols || head >= a.groups) continue;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float v[4] = {value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3)};
+        kv4_emit<T, D>(a, b, h * a.groups + head, split, g * kKv4Group + r * 4, v, ref[c], l[c], g == 0 && r == 0);
+      }
+    }
+  }
+}
+
+// Merges the splits' partials of a row: WPR warps a row, each over every WPR-th partial, lanes over values.
+template <typename T, int D, int WPR>
+__global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4DecodeArgs a) {
+  constexpr int PER = D / 32;
+  using Vec = typename std::conditional<PER == 4, float4, float2>::type;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the split kernel
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + warp / WPR;
+  const int part = warp % WPR;
+  const bool live = row < a.batch * a.hq;
+  const int64_t b = live ? row / a.hq : 0;
+  const int64_t ctx = live ? a.context_lens[b] : 0;
+  const int64_t pages = min(ctx > 0 ? (ctx + a.block_size - 1) / a.block_size : 0, a.max_blocks);
+  const int n = (int)((pages + a.split_pages - 1) / a.split_pages);
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + row * a.max_splits;
+  const float* src = a.ws_o + row * a.max_splits * D + lane * PER;
+  float m_all = -INFINITY;
+  for (int p = lane; p < n; p += 32) m_all = fmaxf(m_all, ml[p].x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, off));
+  float acc[PER], l = 0.f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 8
+  for (int p = part; p < n; p += WPR) {
+    const float2 x = ml[p];
+    const Vec v = *reinterpret_cast<const Vec*>(src + (int64_t)p * D);
+    const float f = m_all == -INFINITY ? 1.f : ex2_approx(x.x - m_all);
+    l = fmaf(f, x.y, l);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) acc[i] = fmaf(f, reinterpret_cast<const float*>(&v)[i], acc[i]);
+  }
+  if constexpr (WPR > 1) {
+    __shared__ float sa[8][D + 1];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sa[warp][lane * PER + i] = acc[i];
+    if (lane == 0) sa[warp][D] = l;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int w = 1; w < WPR; ++w) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) acc[i] += sa[warp + w][lane * PER + i];
+      l += sa[warp + w][D];
+    }
+  }
+  if (!live) return;
+  T* dst = reinterpret_cast<T*>(a.out + b * a.out_sb) + (row - b * a.hq) * D + lane * PER;
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no token: zeros
+#pragma unroll
+  for (int i = 0; i < PER; ++i) dst[i] = Elem<T>::from_f(acc[i] * inv);
 }
 
 template <typename T, int D, int BS, int HB, int SH>
@@ -585,24 +700,16 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess) return e;
-  DecodeArgs d{};
-  d.context_lens = a.context_lens;
-  d.batch = a.batch;
-  d.max_blocks = a.max_blocks;
-  d.hq = a.hq;
-  d.head_dim = D;
-  d.block_size = BS;
-  d.split_pages = a.split_pages;
-  d.parts_per_split = S::kUnits;
-  d.max_parts = a.max_parts;
-  d.ws_o = a.ws_o;
-  d.ws_ml = a.ws_ml;
-  d.out = a.out;
-  d.out_sb = a.out_sb;
-  cfg.gridDim = dim3((unsigned)((a.batch * a.hq + 3) / 4));
-  cfg.blockDim = dim3(128);
+  if (a.max_splits == 1) return cudaSuccess;  // the split kernel wrote the rows
+  const int64_t rows = a.batch * a.hq;
+  cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, decode_combine_kernel<T, D>, d);
+  if (a.max_splits > 16) {
+    cfg.gridDim = dim3((unsigned)rows);
+    return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 8>, a);
+  }
+  cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
+  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 1>, a);
 }
 
 template <typename T, int D, int BS>
@@ -631,16 +738,17 @@ Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int6
               (block_size == 16 || block_size == 32) && groups >= 1 && groups <= 8;
   if (!p.use_mma) return p;
   p.heads_per_cta = (hkv % 4 == 0) ? 4 : (hkv % 2 == 0) ? 2 : 1;
-  p.parts_per_split = kKv4Consumers / p.heads_per_cta;
+  const int64_t units = kKv4Consumers / p.heads_per_cta;  // of 32 tokens in a stage
   // Splits of 1024 tokens x 4 KV heads per CTA, halved while the grid would not cover the SMs twice; at
   // least one unit a warp.
   const int64_t ctas = batch * (hkv / p.heads_per_cta);
-  const int64_t least = p.parts_per_split * (kKv4Unit / block_size);
-  int64_t pages = 1024 * p.parts_per_split / block_size;
+  const int64_t least = units * (kKv4Unit / block_size);
+  int64_t pages = 1024 * units / block_size;
   while (pages > least && ctas * ((max_blocks + pages - 1) / pages) < 2 * 148 * 3) pages /= 2;
   p.split_pages = (int)pages;
   p.max_splits = (int)((max_blocks + p.split_pages - 1) / p.split_pages);
-  const size_t rows = (size_t)batch * hq * p.max_splits * p.parts_per_split;
+  if (p.max_splits == 1) return p;
+  const size_t rows = (size_t)batch * hq * p.max_splits;
   p.ws_bytes = ((rows * head_dim * sizeof(float) + 255) & ~size_t(255)) + ((rows * 8 + 255) & ~size_t(255));
   return p;
 }
