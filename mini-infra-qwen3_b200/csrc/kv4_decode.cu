@@ -353,7 +353,9 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
   constexpr int kTileTok = BS == 16 ? 0 : 16;
   const int my_tile = SH == 2 ? t >> 1 : 0;
   const uint32_t my_par = my_tile * (kTilePage + kTileTok * NG * 4) + kPar + r * NG * 4;
-  const uint32_t col_mask = r < 4 ? 0xffffffffu : 0u;  // SH = 2: the columns of the first tile
+  // SH = 2: ones in the columns of the first tile, and of the second.  Products rather than masks: the
+  // ALU pipe, where the codes are cut, is the busiest.
+  const __half2 ones[2] = {__float2half2_rn(r < 4 ? 1.f : 0.f), __float2half2_rn(r < 4 ? 0.f : 1.f)};
 
   for (int it = 0; it < n_iter; ++it, left -= UN * kKv4Unit) {
     const int st = it % NST;
@@ -519,7 +521,6 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
           for (int i = 0; i < SH; ++i) {
             uint32_t c[4];
             ldmatrix_x4_trans(v_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
-            const uint32_t mask = SH == 1 ? 0xffffffffu : i ? ~col_mask : col_mask;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int g = gp * 2 + j;
@@ -528,11 +529,17 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
               kv4_operands(c[2 * j + 1], hi);
               const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
               const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
-              Mma16816<__half>::run(o[2 * g], a0, pb[j][0] & mask, pb[j][1] & mask);
-              Mma16816<__half>::run(o[2 * g + 1], a1, pb[j][0] & mask, pb[j][1] & mask);
+              uint32_t b[kTwo ? 4 : 2];
+#pragma unroll
+              for (int e = 0; e < (kTwo ? 4 : 2); ++e) {
+                const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&pb[j][e]), ones[i]);
+                b[e] = SH == 1 ? pb[j][e] : *reinterpret_cast<const uint32_t*>(&w);
+              }
+              Mma16816<__half>::run(o[2 * g], a0, b[0], b[1]);
+              Mma16816<__half>::run(o[2 * g + 1], a1, b[0], b[1]);
               if constexpr (kTwo) {
-                Mma16816<__half>::run(o[2 * g], a0, pb[j][2] & mask, pb[j][3] & mask);
-                Mma16816<__half>::run(o[2 * g + 1], a1, pb[j][2] & mask, pb[j][3] & mask);
+                Mma16816<__half>::run(o[2 * g], a0, b[2], b[3]);
+                Mma16816<__half>::run(o[2 * g + 1], a1, b[2], b[3]);
               }
             }
           }
