@@ -211,12 +211,15 @@ int mi_kv4_paged_decode(const void* q, const int64_t* q_strides, const void* k_n
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = static_cast<char*>(out);
   a.out_sb = out_stride * es;
-  a.split_pages = plan.split_pages;
-  a.max_splits = plan.max_splits;
+  a.ctas = plan.ctas;
+  a.whole = plan.whole;
+  a.min_steps = plan.min_steps;
+  a.part_rows = plan.part_rows;
   if (plan.ws_bytes) {
-    const size_t o_bytes = (size_t)batch * num_q_heads * a.max_splits * head_dim * sizeof(float);
-    a.ws_o = static_cast<float*>(workspace);
-    a.ws_ml = reinterpret_cast<float*>(static_cast<char*>(workspace) + ((o_bytes + 255) & ~size_t(255)));
+    char* ws = static_cast<char*>(workspace);
+    a.ws_o = reinterpret_cast<float*>(ws);
+    a.ws_ml = reinterpret_cast<float*>(ws + plan.o_bytes);
+    a.cuts = reinterpret_cast<mi::Kv4Cut*>(ws + plan.o_bytes + plan.ml_bytes);
   }
   cudaError_t e = mi::launch_kv4_decode(a, plan, dtype, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? MI_OK : cuda_fail(e, "mi_kv4_paged_decode launch");

@@ -284,17 +284,29 @@ struct Kv4DecodeArgs {
   char* out;
   int64_t out_sb;  // bytes
   // tensor-core path
-  int split_pages;  // pages handled by one split
-  int max_splits;   // grid.x; 1: the split kernel writes the rows
-  float* ws_o;      // [batch, hq, max_splits, head_dim] partial sums
-  float* ws_ml;     // [batch, hq, max_splits, 2] their references and sums of weights
+  int ctas;          // persistent CTAs of the split kernel
+  int whole;         // CTAs take whole sequences: nothing to combine
+  int min_steps;     // steps of a CTA, at least
+  int part_rows;     // query heads of one CTA's KV heads
+  float* ws_o;       // [ctas, 2, part_rows, head_dim] partial sums
+  float* ws_ml;      // [ctas, 2, part_rows, 2] their references and sums of weights
+  struct Kv4Cut* cuts;  // [ctas]
+};
+// The sequence that a CTA of the split kernel starts and others finish (pieces == 0: none).
+struct Kv4Cut {
+  int64_t b;
+  int hb;      // block of KV heads
+  int slot;    // of the first piece in its CTA
+  int pieces;  // consecutive CTAs that hold a part
 };
 struct Kv4DecodePlan {
   bool use_mma;
+  bool whole;
   int heads_per_cta;
-  int split_pages;
-  int max_splits;
-  size_t ws_bytes;
+  int part_rows;
+  int min_steps;
+  int ctas;
+  size_t o_bytes, ml_bytes, ws_bytes;
 };
 Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int64_t max_blocks, int block_size,
                               int dtype);

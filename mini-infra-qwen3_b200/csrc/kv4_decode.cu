@@ -121,20 +121,24 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_decode_generic_kernel(cons
 
 constexpr int kKv4Consumers = 4;  // consumer warps of the tensor-core kernel's CTA
 constexpr int kKv4SplitThreads = (kKv4Consumers + 1) * 32;
-constexpr int kKv4Smem = 62 * 1024;  // three CTAs per SM
-
+constexpr int kKv4CtasPerSm = 3;
+constexpr int kKv4Smem = 74 * 1024;  // of a CTA
+constexpr int kKv4MinSteps = 2;    // steps of a CTA, at least
+constexpr int kKv4WholeSteps = 8;  // sequences of at most this many are not cut
 constexpr int kKv4Unit = 32;  // tokens a consumer warp takes at a time: two 16-row tiles
 
-template <int D, int BS, int HB>
+template <int D, int BS, int HB, int SH>
 struct Kv4Shape {
   static constexpr int kGroups = D / kKv4Group;
-  static constexpr int kUnits = kKv4Consumers / HB;     // units of a stage: one (KV head, unit) per warp
-  static constexpr int kUnitPages = kKv4Unit / BS;
-  static constexpr int kPages = kUnits * kUnitPages;    // pages of a stage
+  static constexpr int kCols = 8 / SH;                  // query heads of a KV head, rounded up
+  static constexpr int kUnits = kKv4Consumers / HB;     // units of a step: one (KV head, unit) per warp
+  static constexpr int kTokens = kUnits * kKv4Unit;     // tokens of a step
+  static constexpr int kPages = kTokens / BS;           // and its pages
   static constexpr int kPageBytes = BS * D / 2 + BS * kGroups * 4;
   static constexpr int kStageBytes = kPages * HB * 2 * kPageBytes;
-  static constexpr int kStages = std::max(2, std::min(8, kKv4Smem / kStageBytes));
-  static constexpr int kSmemBytes = kStages * (kStageBytes + 16) + 128;
+  static constexpr int kMergeBytes = kUnits > 1 ? kKv4Consumers * kCols * (D + 2) * 4 : 0;
+  static constexpr int kStages = std::min(6, (kKv4Smem - kMergeBytes - 128) / (kStageBytes + 16));
+  static constexpr int kSmemBytes = kMergeBytes + kStages * (kStageBytes + 16) + 128;
 };
 
 constexpr float kKv4TopLog2 = 11.f;   // p * s of a new reference: at most 2^11
@@ -164,114 +168,241 @@ __device__ __forceinline__ void kv4_params(const uint8_t* p, uint32_t (&w)[NG]) 
   }
 }
 
-// Four values of a row's sum, relative to ref, with the sum l of its weights: the output where the row has
-// one split, else the split's partial.
+// Where a CTA's share of the work lies.  The sequences (row b, block of HB KV heads), one after the other,
+// are a stream of steps; CTA c takes steps [c * quota, (c + 1) * quota).  A sequence of no tokens has one
+// step, which writes its zeros.
+struct Kv4Walk {
+  int64_t b;
+  int64_t rest;  // steps left to this CTA, the current sequence's included
+  int hb;
+  int pos;       // first step of the current sequence that is this CTA's
+  int steps;     // of the current sequence
+  int ctx;       // tokens of the current sequence
+  __device__ __forceinline__ int take() const { return (int)min(rest, (int64_t)(steps - pos)); }
+};
+
+template <int TOKENS>
+__device__ __forceinline__ int kv4_steps(int ctx) {
+  return max(1, (ctx + TOKENS - 1) / TOKENS);
+}
+
+// Tokens of row b, at most what its block table covers.
+__device__ __forceinline__ int kv4_ctx(const Kv4DecodeArgs& a, int64_t b) {
+  return (int)max((int64_t)0, min(a.context_lens[b], a.max_blocks * a.block_size));
+}
+
+template <int TOKENS>
+__device__ __forceinline__ void kv4_advance(const Kv4DecodeArgs& a, Kv4Walk& w, int heads_per_cta, int next_ctx) {
+  w.rest -= w.take();
+  w.pos = 0;
+  if (++w.hb * heads_per_cta == a.hkv) {
+    w.hb = 0;
+    ++w.b;
+    w.ctx = next_ctx;
+    w.steps = kv4_steps<TOKENS>(next_ctx);
+  }
+}
+
+// This CTA's start, by every thread: a block-wide scan over the rows' steps.  False where it has none.
+template <int TOKENS>
+__device__ bool kv4_start(const Kv4DecodeArgs& a, int heads_per_cta, Kv4Walk& w, int64_t& quota) {
+  __shared__ int64_t s_sum[kKv4SplitThreads / 32];
+  __shared__ Kv4Walk s_walk;
+  const int nhb = a.hkv / heads_per_cta;
+  if (a.whole) {  // whole sequences: no scan
+    const int64_t n = a.batch * nhb;
+    const int64_t first = blockIdx.x * n / gridDim.x, last = (blockIdx.x + 1) * n / gridDim.x;
+    if (first >= last) return false;
+    w.b = first / nhb;
+    w.hb = (int)(first - w.b * nhb);
+    w.pos = 0;
+    w.ctx = kv4_ctx(a, w.b);
+    w.steps = kv4_steps<TOKENS>(w.ctx);
+    w.rest = 0;  // counted in steps: filled in below
+    for (int64_t q = first; q < last; ++q) w.rest += kv4_steps<TOKENS>(q / nhb == w.b ? w.ctx : kv4_ctx(a, q / nhb));
+    quota = 0;
+    return true;
+  }
+  const int64_t per = (a.batch + kKv4SplitThreads - 1) / kKv4SplitThreads;
+  const int64_t b0 = min(a.batch, per * threadIdx.x), b1 = min(a.batch, b0 + per);
+  int64_t mine = 0;
+  for (int64_t b = b0; b < b1; ++b) mine += (int64_t)nhb * kv4_steps<TOKENS>(kv4_ctx(a, b));
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t scan = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan += up;
+  }
+  if (lane == 31) s_sum[warp] = scan;
+  __syncthreads();
+  int64_t total = 0, before = scan - mine;
+  for (int i = 0; i < kKv4SplitThreads / 32; ++i) {
+    if (i < warp) before += s_sum[i];
+    total += s_sum[i];
+  }
+  quota = max((int64_t)a.min_steps, (total + gridDim.x - 1) / gridDim.x);
+  const int64_t first = quota * blockIdx.x;
+  if (first >= total) return false;
+  if (first >= before && first < before + mine) {  // one thread's rows hold the start
+    int64_t at = before;
+    for (int64_t b = b0; b < b1; ++b) {
+      const int ctx = kv4_ctx(a, b);
+      const int steps = kv4_steps<TOKENS>(ctx);
+      if (first < at + (int64_t)nhb * steps) {
+        const int64_t in = first - at;
+        s_walk.b = b;
+        s_walk.rest = min(quota, total - first);
+        s_walk.hb = (int)(in / steps);
+        s_walk.pos = (int)(in - (int64_t)s_walk.hb * steps);
+        s_walk.steps = steps;
+        s_walk.ctx = ctx;
+        break;
+      }
+      at += (int64_t)nhb * steps;
+    }
+  }
+  __syncthreads();
+  w = s_walk;
+  return true;
+}
+
+// Four values of a row's sum, relative to ref, with the sum l of its weights: the output where this CTA had
+// the whole sequence (slot < 0), else one of the CTA's two partials.
 template <typename T, int D>
-__device__ __forceinline__ void kv4_emit(const Kv4DecodeArgs& a, int64_t b, int hq, int split, int d, const float (&v)[4],
-                                         float ref, float l, bool first) {
-  if (a.max_splits == 1) {
+__device__ __forceinline__ void kv4_emit(const Kv4DecodeArgs& a, int64_t b, int hq, int slot, int row, int d,
+                                         const float (&v)[4], float ref, float l, bool first) {
+  if (slot < 0) {
     T* dst = reinterpret_cast<T*>(a.out + b * a.out_sb) + (int64_t)hq * D + d;
     const float inv = 1.f / l;
 #pragma unroll
     for (int i = 0; i < 4; ++i) dst[i] = Elem<T>::from_f(v[i] * inv);
     return;
   }
-  const int64_t idx = (b * a.hq + hq) * a.max_splits + split;
+  const int64_t idx = ((int64_t)blockIdx.x * 2 + slot) * a.part_rows + row;
   *reinterpret_cast<float4*>(a.ws_o + idx * D + d) = make_float4(v[0], v[1], v[2], v[3]);
   if (first) *reinterpret_cast<float2*>(a.ws_ml + idx * 2) = make_float2(ref, l);
 }
 
 template <typename T, int D, int BS, int HB, int SH>
-__global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(const Kv4DecodeArgs a) {
-  using S = Kv4Shape<D, BS, HB>;
+__global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_split_kernel(const Kv4DecodeArgs a) {
+  using S = Kv4Shape<D, BS, HB, SH>;
   constexpr int NG = S::kGroups;
   constexpr int NST = S::kStages;
   constexpr int PG = S::kPages;
   constexpr int UN = S::kUnits;
+  constexpr int kCols = S::kCols;
   constexpr bool kTwo = std::is_same<T, __half>::value;  // p * s as two fp16 operands
+  static_assert(NST >= 2, "a ring");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the append
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + NST * S::kStageBytes);
+  float* merge = reinterpret_cast<float*>(smem + NST * S::kStageBytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + NST * S::kStageBytes + S::kMergeBytes);
   uint64_t* empty_bar = full_bar + NST;
 
-  const int split = blockIdx.x;
-  const int head0 = blockIdx.y * HB;
-  const int64_t b = blockIdx.z;
-  int64_t ctx = a.context_lens[b];
-  int64_t n_pages = ctx > 0 ? (ctx + BS - 1) / BS : 0;
-  if (n_pages > a.max_blocks) {
-    if (threadIdx.x == 0 && split == 0) record_status(MI_STATUS_BAD_LENGTH);
-    n_pages = a.max_blocks;
-    ctx = n_pages * BS;
-  }
-  const int64_t page_begin = (int64_t)split * a.split_pages;
-  if (page_begin >= n_pages) {  // uniform for the CTA
-    if (a.max_splits == 1)  // a row of no tokens that no combine follows
-      for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4SplitThreads)
-        reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
-    return;
-  }
-  const int64_t page_end = min(n_pages, page_begin + (int64_t)a.split_pages);
-  const int n_iter = (int)((page_end - page_begin + PG - 1) / PG);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
+  if (blockIdx.x == 0)
+    for (int64_t b = threadIdx.x; b < a.batch; b += kKv4SplitThreads)
+      if (a.context_lens[b] > a.max_blocks * a.block_size) record_status(MI_STATUS_BAD_LENGTH);
+  Kv4Walk w;
+  int64_t quota;
   if (threadIdx.x == 0) {
+    if (a.cuts) a.cuts[blockIdx.x].pieces = 0;
     for (int i = 0; i < NST; ++i) {
       mbar_init(&full_bar[i], 1);
       mbar_init(&empty_bar[i], kKv4Consumers);
     }
     fence_mbar_init();
   }
+  if (!kv4_start<S::kTokens>(a, HB, w, quota)) return;  // uniform for the CTA
   __syncthreads();
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int nhb = a.hkv / HB;
   bool aborted = false;
+  int st = 0, phase = 0;  // of the ring
 
   if (warp == kKv4Consumers) {
-    // ---------------- producer: lane 2p + kv copies K or V of page p of a stage ----------------
+    // ---------------- producer: lane 2p + kv copies K or V of page p of a step ----------------
     constexpr uint32_t kBytes = HB * S::kPageBytes;
     const int my_page = lane >> 1;
     const bool mine = my_page < PG;
-    const char* pool = ((lane & 1) ? a.v_pool : a.k_pool) + (int64_t)head0 * S::kPageBytes;
+    const char* pool = (lane & 1) ? a.v_pool : a.k_pool;
     const int64_t block_bytes = (int64_t)a.hkv * S::kPageBytes;
-    const int64_t* table = a.block_tables + b * a.table_stride;
-    int64_t next_blk = 0;  // each lane reads its next block id one stage ahead
-    if (mine && page_begin + my_page < page_end) next_blk = table[page_begin + my_page];
-    for (int it = 0; it < n_iter; ++it) {
-      const int st = it % NST;
-      if (it >= NST) {
-        mbar_wait(&empty_bar[st], ((it / NST) - 1) & 1, aborted);
-        aborted = __any_sync(0xffffffffu, aborted);
-      }
-      const int64_t first = page_begin + (int64_t)it * PG;
-      const int npg = (int)min((int64_t)PG, page_end - first);
-      int64_t blk = next_blk;
-      const int64_t ahead = first + PG + my_page;
-      if (mine && it + 1 < n_iter && ahead < page_end) next_blk = table[ahead];
-      if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], (uint32_t)npg * 2 * kBytes);
-      __syncwarp();
-      if (mine && my_page < npg) {
-        if (blk < 0 || blk >= a.num_blocks) {
-          record_status(MI_STATUS_BAD_BLOCK);
-          blk = 0;  // the null block
+    const int64_t* table = a.block_tables + w.b * a.table_stride;
+    int n_pages = (w.ctx + BS - 1) / BS;
+    int64_t next_blk = 0;  // each lane reads its block id one step ahead, across sequences too
+    if (mine && w.pos * PG + my_page < n_pages) next_blk = table[w.pos * PG + my_page];
+    while (true) {
+      const int n = w.take();
+      const bool more = w.rest > n;
+      const bool next_row = (w.hb + 1) == nhb;
+      const int next_ctx = more ? (next_row ? kv4_ctx(a, w.b + 1) : w.ctx) : 0;
+      const int64_t* next_table = table + (next_row ? a.table_stride : 0);
+      const int64_t head_off = (int64_t)w.hb * kBytes;
+      for (int s = 0; s < n; ++s) {
+        const int first = (w.pos + s) * PG;
+        const int npg = min(PG, n_pages - first);
+        int64_t blk = next_blk;
+        if (s + 1 < n) {
+          if (mine && first + PG + my_page < n_pages) next_blk = table[first + PG + my_page];
+        } else if (more) {
+          if (mine && my_page * BS < next_ctx) next_blk = next_table[my_page];
         }
-        bulk_load(smem + st * S::kStageBytes + lane * kBytes, pool + blk * block_bytes, kBytes, &full_bar[st]);
+        if (npg <= 0) continue;  // a sequence of no tokens
+        mbar_wait(&empty_bar[st], phase ^ 1, aborted);
+        aborted = __any_sync(0xffffffffu, aborted);
+        if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], (uint32_t)npg * 2 * kBytes);
+        __syncwarp();
+        if (mine && my_page < npg) {
+          if (blk < 0 || blk >= a.num_blocks) {
+            record_status(MI_STATUS_BAD_BLOCK);
+            blk = 0;  // the null block
+          }
+          bulk_load(smem + st * S::kStageBytes + lane * kBytes, pool + blk * block_bytes + head_off, kBytes,
+                    &full_bar[st]);
+        }
+        if (++st == NST) st = 0, phase ^= 1;
       }
+      if (!more) return;
+      kv4_advance<S::kTokens>(a, w, HB, next_ctx);
+      table = a.block_tables + w.b * a.table_stride;
+      n_pages = (w.ctx + BS - 1) / BS;
     }
-    return;
   }
 
   // ---------------- consumers: one warp per (KV head, unit of 32 tokens) ----------------
   const int hl = warp / UN;
   const int un = warp % UN;
-  const int h = head0 + hl;
-  const int r = lane >> 2;  // MMA row (token or value) and, of a B operand, its column (query head)
+  const int r = lane >> 2;  // MMA row (token or value) and, of a B operand, its column
   const int t = lane & 3;
+  // rows of the 8x8 matrices: (token octet, 16 bytes of a group) x two groups
+  const uint32_t mat_row = (uint32_t)(((lane >> 3) & 1) * 8 + (lane & 7) + (lane >> 4) * BS) * 16;
+  constexpr uint32_t kPar = BS * D / 2;  // of a page
+  const uint32_t k_off = (un * (kKv4Unit / BS) * 2 * HB + hl) * S::kPageBytes;
+  // The unit's two tiles: tile i's K page and the token offset in it (V pages lie HB pages further); and
+  // the tile of this lane's weights, which are one set of four for both tiles (SH = 2) or one for each.
+  constexpr int kSets = 2 / SH;
+  constexpr int kTilePage = BS == 16 ? 2 * HB * S::kPageBytes : 0;
+  constexpr int kTileTok = BS == 16 ? 0 : 16;
+  const int my_tile = SH == 2 ? t >> 1 : 0;
+  const uint32_t my_par = my_tile * (kTilePage + kTileTok * NG * 4) + kPar + r * NG * 4;
+  // SH = 2: ones in the columns of the first tile, and of the second.  Products rather than masks: the
+  // ALU pipe, where the codes are cut, is the busiest.
+  const __half2 ones[2] = {__float2half2_rn(r < 4 ? 1.f : 0.f), __float2half2_rn(r < 4 ? 0.f : 1.f)};
+
+  for (int64_t done = 0;; ) {  // one sequence's share at a time; `done`: steps of this CTA before it
+  const int n_steps = w.take();
+  const bool more = w.rest > n_steps;
+  const int next_ctx = more ? (w.hb + 1 == nhb ? kv4_ctx(a, w.b + 1) : w.ctx) : 0;
+  const int64_t b = w.b;
+  const int head0 = w.hb * HB;
+  const int h = head0 + hl;
+  int left = min(w.ctx - w.pos * S::kTokens, n_steps * S::kTokens) - un * kKv4Unit;  // tokens from this unit on
 
   // q as the B operand of S^T: this lane holds column r's values d = 32 g + 8 t + 0..7 of every group.
   // Column c is query head c % kCols; with SH = 2 the first four columns are for the first tile's
   // tokens, the last four for the second's.
-  constexpr int kCols = 8 / SH;
   uint32_t qb[NG][4];
   uint32_t mb[3];  // B operands of the minimum term, see below
   float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: columns 2t, 2t + 1
@@ -340,26 +471,8 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
 #pragma unroll
   for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
 
-  // rows of the 8x8 matrices: (token octet, 16 bytes of a group) x two groups
-  const uint32_t mat_row = (uint32_t)(((lane >> 3) & 1) * 8 + (lane & 7) + (lane >> 4) * BS) * 16;
-  constexpr uint32_t kPar = BS * D / 2;  // of a page
-  const uint32_t k_off = (un * S::kUnitPages * 2 * HB + hl) * S::kPageBytes;
-  int left = (int)(min(ctx, page_end * BS) - page_begin * BS) - un * kKv4Unit;  // tokens from this unit on
-
-  // The unit's two tiles: tile i's K page and the token offset in it (V pages lie HB pages further); and
-  // the tile of this lane's weights, which are one set of four for both tiles (SH = 2) or one for each.
-  constexpr int kSets = 2 / SH;
-  constexpr int kTilePage = BS == 16 ? 2 * HB * S::kPageBytes : 0;
-  constexpr int kTileTok = BS == 16 ? 0 : 16;
-  const int my_tile = SH == 2 ? t >> 1 : 0;
-  const uint32_t my_par = my_tile * (kTilePage + kTileTok * NG * 4) + kPar + r * NG * 4;
-  // SH = 2: ones in the columns of the first tile, and of the second.  Products rather than masks: the
-  // ALU pipe, where the codes are cut, is the busiest.
-  const __half2 ones[2] = {__float2half2_rn(r < 4 ? 1.f : 0.f), __float2half2_rn(r < 4 ? 0.f : 1.f)};
-
-  for (int it = 0; it < n_iter; ++it, left -= UN * kKv4Unit) {
-    const int st = it % NST;
-    mbar_wait(&full_bar[st], (it / NST) & 1, aborted);
+  for (int it = w.ctx > 0 ? n_steps : 0; it > 0; --it, left -= S::kTokens) {
+    mbar_wait(&full_bar[st], phase, aborted);
     if (left > 0) {
       const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
       const uint32_t k_mat = smem_u32(k_unit) + mat_row;
@@ -548,6 +661,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty_bar[st]);
+    if (++st == NST) st = 0, phase ^= 1;
   }
 
   if constexpr (SH == 2) {
@@ -586,12 +700,24 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
     }
   }
   auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
-  if constexpr (UN > 1) {
-    // The warps of a KV head merge in shared memory; every stage has been consumed.
-    float* so = reinterpret_cast<float*>(smem);                    // [warp][column][D]
-    float* sml = so + kKv4Consumers * kCols * D;                   // [warp][column](ref, l)
-    static_assert((kKv4Consumers * kCols * (D + 2)) * 4 <= NST * S::kStageBytes, "the merge fits the ring");
-    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");
+  // The rows' outputs where all of the sequence was here, else a partial: slot 0 the CTA's first, 1 its last.
+  const int slot = w.pos == 0 && n_steps == w.steps ? -1 : done > 0;
+  if (slot >= 0 && w.pos == 0 && threadIdx.x == 0) {  // the sequence starts here and is cut: say how often
+    Kv4Cut cut;
+    cut.b = b;
+    cut.hb = w.hb;
+    cut.slot = slot;
+    const int64_t at = blockIdx.x * quota + done;
+    cut.pieces = (int)((at + w.steps - 1) / quota - blockIdx.x) + 1;
+    a.cuts[blockIdx.x] = cut;
+  }
+  if (w.ctx == 0) {  // a row of no tokens
+    for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4Consumers * 32)
+      reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
+  } else if constexpr (UN > 1) {
+    // the warps of a KV head merge in shared memory
+    float* so = merge;                             // [warp][column][D]
+    float* sml = so + kKv4Consumers * kCols * D;   // [warp][column](ref, l)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int col = warp * kCols + 2 * t + c;
@@ -617,11 +743,12 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
         const int col = (hm * UN + u) * kCols + head;
         const float f = m_all == -INFINITY ? 1.f : ex2_approx(sml[2 * col] - m_all);
         l_all = fmaf(f, sml[2 * col + 1], l_all);
-        const float4 w = *reinterpret_cast<const float4*>(so + col * D + d);
-        v[0] = fmaf(f, w.x, v[0]), v[1] = fmaf(f, w.y, v[1]), v[2] = fmaf(f, w.z, v[2]), v[3] = fmaf(f, w.w, v[3]);
+        const float4 x = *reinterpret_cast<const float4*>(so + col * D + d);
+        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
       }
-      kv4_emit<T, D>(a, b, (head0 + hm) * a.groups + head, split, d, v, m_all, l_all, d == 0);
+      kv4_emit<T, D>(a, b, (head0 + hm) * a.groups + head, slot, row, d, v, m_all, l_all, d == 0);
     }
+    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");  // before the next sequence's sums
   } else {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -630,68 +757,72 @@ __global__ void __launch_bounds__(kKv4SplitThreads, 3) kv4_decode_split_kernel(c
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float v[4] = {value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3)};
-        kv4_emit<T, D>(a, b, h * a.groups + head, split, g * kKv4Group + r * 4, v, ref[c], l[c], g == 0 && r == 0);
+        kv4_emit<T, D>(a, b, h * a.groups + head, slot, hl * a.groups + head, g * kKv4Group + r * 4, v, ref[c], l[c],
+                       g == 0 && r == 0);
       }
     }
   }
+  if (!more) return;
+  done += n_steps;
+  kv4_advance<S::kTokens>(a, w, HB, next_ctx);
+  }
 }
 
-// Merges the splits' partials of a row: WPR warps a row, each over every WPR-th partial, lanes over values.
-template <typename T, int D, int WPR>
+// Merges the partials of the sequence that CTA blockIdx.x of the split kernel started and did not finish:
+// four warps a row, each over every fourth piece, lanes over values.
+template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4DecodeArgs a) {
-  constexpr int PER = D / 32;
+  constexpr int PER = D / 32, WPR = 4;
   using Vec = typename std::conditional<PER == 4, float4, float2>::type;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the split kernel
+  const Kv4Cut cut = a.cuts[blockIdx.x];
+  if (cut.pieces == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * (8 / WPR) + warp / WPR;
+  const int row = blockIdx.y * (8 / WPR) + warp / WPR;
   const int part = warp % WPR;
-  const bool live = row < a.batch * a.hq;
-  const int64_t b = live ? row / a.hq : 0;
-  const int64_t ctx = live ? a.context_lens[b] : 0;
-  const int64_t pages = min(ctx > 0 ? (ctx + a.block_size - 1) / a.block_size : 0, a.max_blocks);
-  const int n = (int)((pages + a.split_pages - 1) / a.split_pages);
-  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml) + row * a.max_splits;
-  const float* src = a.ws_o + row * a.max_splits * D + lane * PER;
+  const bool live = row < a.part_rows;
+  // piece i: CTA blockIdx.x + i, in its first slot but for the first piece
+  const int64_t first = ((int64_t)blockIdx.x * 2 + cut.slot) * a.part_rows + (live ? row : 0);
+  const int64_t second = ((int64_t)blockIdx.x * 2 + 2) * a.part_rows + (live ? row : 0);
+  auto at = [&](int i) { return i == 0 ? first : second + (int64_t)(i - 1) * 2 * a.part_rows; };
+  const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
   float m_all = -INFINITY;
-  for (int p = lane; p < n; p += 32) m_all = fmaxf(m_all, ml[p].x);
+  for (int i = lane; i < cut.pieces; i += 32) m_all = fmaxf(m_all, ml[at(i)].x);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, off));
   float acc[PER], l = 0.f;
 #pragma unroll
   for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 8
-  for (int p = part; p < n; p += WPR) {
-    const float2 x = ml[p];
-    const Vec v = *reinterpret_cast<const Vec*>(src + (int64_t)p * D);
+#pragma unroll 4
+  for (int i = part; i < cut.pieces; i += WPR) {
+    const float2 x = ml[at(i)];
+    const Vec v = *reinterpret_cast<const Vec*>(a.ws_o + at(i) * D + lane * PER);
     const float f = m_all == -INFINITY ? 1.f : ex2_approx(x.x - m_all);
     l = fmaf(f, x.y, l);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) acc[i] = fmaf(f, reinterpret_cast<const float*>(&v)[i], acc[i]);
+    for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], acc[e]);
   }
-  if constexpr (WPR > 1) {
-    __shared__ float sa[8][D + 1];
+  __shared__ float sa[8][D + 1];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sa[warp][lane * PER + i] = acc[i];
-    if (lane == 0) sa[warp][D] = l;
-    __syncthreads();
-    if (part != 0) return;
+  for (int e = 0; e < PER; ++e) sa[warp][lane * PER + e] = acc[e];
+  if (lane == 0) sa[warp][D] = l;
+  __syncthreads();
+  if (part != 0 || !live) return;
 #pragma unroll
-    for (int w = 1; w < WPR; ++w) {
+  for (int i = 1; i < WPR; ++i) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) acc[i] += sa[warp + w][lane * PER + i];
-      l += sa[warp + w][D];
-    }
+    for (int e = 0; e < PER; ++e) acc[e] += sa[warp + i][lane * PER + e];
+    l += sa[warp + i][D];
   }
-  if (!live) return;
-  T* dst = reinterpret_cast<T*>(a.out + b * a.out_sb) + (row - b * a.hq) * D + lane * PER;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no token: zeros
+  T* dst = reinterpret_cast<T*>(a.out + cut.b * a.out_sb) + ((int64_t)cut.hb * a.part_rows + row) * D + lane * PER;
+  const float inv = 1.f / l;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) dst[i] = Elem<T>::from_f(acc[i] * inv);
+  for (int e = 0; e < PER; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
 }
 
 template <typename T, int D, int BS, int HB, int SH>
 cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
-  using S = Kv4Shape<D, BS, HB>;
+  using S = Kv4Shape<D, BS, HB, SH>;
   auto kern = kv4_decode_split_kernel<T, D, BS, HB, SH>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmemBytes);
   if (e != cudaSuccess) return e;
@@ -699,24 +830,18 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)a.max_splits, (unsigned)(a.hkv / HB), (unsigned)a.batch);
+  cfg.gridDim = dim3((unsigned)a.ctas);
   cfg.blockDim = dim3(kKv4SplitThreads);
   cfg.dynamicSmemBytes = S::kSmemBytes;
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
-  if (e != cudaSuccess) return e;
-  if (a.max_splits == 1) return cudaSuccess;  // the split kernel wrote the rows
-  const int64_t rows = a.batch * a.hq;
+  if (e != cudaSuccess || a.whole) return e;
+  cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)((a.part_rows + 1) / 2));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  if (a.max_splits > 16) {
-    cfg.gridDim = dim3((unsigned)rows);
-    return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 8>, a);
-  }
-  cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
-  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 1>, a);
+  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, a);
 }
 
 template <typename T, int D, int BS>
@@ -745,18 +870,19 @@ Kv4DecodePlan plan_kv4_decode(int64_t batch, int hq, int hkv, int head_dim, int6
               (block_size == 16 || block_size == 32) && groups >= 1 && groups <= 8;
   if (!p.use_mma) return p;
   p.heads_per_cta = (hkv % 4 == 0) ? 4 : (hkv % 2 == 0) ? 2 : 1;
-  const int64_t units = kKv4Consumers / p.heads_per_cta;  // of 32 tokens in a stage
-  // Splits of 1024 tokens x 4 KV heads per CTA, halved while the grid would not cover the SMs twice; at
-  // least one unit a warp.
-  const int64_t ctas = batch * (hkv / p.heads_per_cta);
-  const int64_t least = units * (kKv4Unit / block_size);
-  int64_t pages = 1024 * units / block_size;
-  while (pages > least && ctas * ((max_blocks + pages - 1) / pages) < 2 * 148 * 3) pages /= 2;
-  p.split_pages = (int)pages;
-  p.max_splits = (int)((max_blocks + p.split_pages - 1) / p.split_pages);
-  if (p.max_splits == 1) return p;
-  const size_t rows = (size_t)batch * hq * p.max_splits;
-  p.ws_bytes = ((rows * head_dim * sizeof(float) + 255) & ~size_t(255)) + ((rows * 8 + 255) & ~size_t(255));
+  const int64_t step_tokens = kKv4Consumers / p.heads_per_cta * kKv4Unit;
+  const int64_t sequences = batch * (hkv / p.heads_per_cta);
+  const int64_t steps = (max_blocks * block_size + step_tokens - 1) / step_tokens;  // of the longest sequence, at most
+  const int64_t ctas = 148 * kKv4CtasPerSm;
+  p.part_rows = p.heads_per_cta * groups;
+  p.min_steps = kKv4MinSteps;
+  p.whole = steps <= kKv4WholeSteps;
+  p.ctas = (int)std::min<int64_t>(ctas, p.whole ? sequences : (sequences * steps + p.min_steps - 1) / p.min_steps);
+  if (p.whole) return p;
+  const size_t rows = (size_t)p.ctas * 2 * p.part_rows;
+  p.o_bytes = (rows * head_dim * sizeof(float) + 255) & ~size_t(255);
+  p.ml_bytes = (rows * 2 * sizeof(float) + 255) & ~size_t(255);
+  p.ws_bytes = p.o_bytes + p.ml_bytes + (((size_t)p.ctas * sizeof(Kv4Cut) + 255) & ~size_t(255));
   return p;
 }
 
