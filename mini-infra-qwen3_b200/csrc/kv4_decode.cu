@@ -478,10 +478,10 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
       const uint32_t k_mat = smem_u32(k_unit) + mat_row;
       const uint32_t v_mat = k_mat + HB * S::kPageBytes;
       const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
-      // ---- scores: x[n][0..1] token r, [2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
-      float x[kSets][4], wide[kSets][2];
 #pragma unroll
       for (int n = 0; n < kSets; ++n) {
+        // ---- scores: x[0..1] token r, x[2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
+        float x[4], wide[2];
         const uint8_t* k_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4);
         uint32_t kw[2][NG];
         kv4_params<NG>(k_par, kw[0]);
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[n][j] = fmaf(s[j], unit[j & 1], y[j]);
+        for (int j = 0; j < 4; ++j) x[j] = fmaf(s[j], unit[j & 1], y[j]);
         // widest step of each token (positive bfloat16s order as integers)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -540,63 +540,48 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
           uint32_t w = vw[0];
 #pragma unroll
           for (int g = 1; g < NG; ++g) w = __vmaxu2(w, vw[g]);
-          wide[n][j] = fmaxf(kv4_step(w), kKv4Narrow);
+          wide[j] = fmaxf(kv4_step(w), kKv4Narrow);
         }
         if (tail) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             if ((n + my_tile) * 16 + j * 8 + r >= left) {
-              x[n][2 * j] = x[n][2 * j + 1] = -INFINITY;
-              wide[n][j] = kKv4Narrow;
+              x[2 * j] = x[2 * j + 1] = -INFINITY;
+              wide[j] = kKv4Narrow;
             }
         }
-      }
-      // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
-      // then to where the largest p * s of this unit is 2^11 ----
-      float p[kSets][4];
-      float most = 0.f;
+        // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
+        // then to where the largest p * s of these tokens is 2^11 ----
+        float p[4];
 #pragma unroll
-      for (int n = 0; n < kSets; ++n) {
+        for (int j = 0; j < 4; ++j) p[j] = ex2_approx(x[j] - ref[j & 1]);
+        const float most = fmaxf(fmaxf(p[0], p[1]) * wide[0], fmaxf(p[2], p[3]) * wide[1]);
+        if (__any_sync(0xffffffffu, most > kKv4Limit)) {
+          const float wl[2] = {log2f(wide[0]) - kKv4TopLog2, log2f(wide[1]) - kKv4TopLog2};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[n][j] = ex2_approx(x[n][j] - ref[j & 1]);
-        most = fmaxf(most, fmaxf(fmaxf(p[n][0], p[n][1]) * wide[n][0], fmaxf(p[n][2], p[n][3]) * wide[n][1]));
-      }
-      if (__any_sync(0xffffffffu, most > kKv4Limit)) {
-        float ask[2] = {-INFINITY, -INFINITY};
+          for (int c = 0; c < 2; ++c) {
+            float want = fmaxf(x[c] + wl[0], x[c + 2] + wl[1]);
 #pragma unroll
-        for (int n = 0; n < kSets; ++n)
+            for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
+            want = fmaxf(want, ref[c]);
+            const float base = want == -INFINITY ? 0.f : want;
+            const float alpha = ex2_approx(ref[c] - base);  // 0 from the initial -inf
+            l[c] *= alpha;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            ask[j & 1] = fmaxf(ask[j & 1], x[n][j] + (log2f(wide[n][j >> 1]) - kKv4TopLog2));
+            for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float want = ask[c];
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
-          want = fmaxf(want, ref[c]);
-          const float base = want == -INFINITY ? 0.f : want;
-          const float alpha = ex2_approx(ref[c] - base);  // 0 from the initial -inf
-          l[c] *= alpha;
-#pragma unroll
-          for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            o[i][c] *= alpha;
-            o[i][c + 2] *= alpha;
+            for (int i = 0; i < D / 16; ++i) {
+              o[i][c] *= alpha;
+              o[i][c + 2] *= alpha;
+            }
+            p[c] = ex2_approx(x[c] - base);
+            p[c + 2] = ex2_approx(x[c + 2] - base);
+            ref[c] = want;
           }
-#pragma unroll
-          for (int n = 0; n < kSets; ++n) {
-            p[n][c] = ex2_approx(x[n][c] - base);
-            p[n][c + 2] = ex2_approx(x[n][c + 2] - base);
-          }
-          ref[c] = want;
         }
-      }
-      // ---- O^T += V^T (p s)^T, z += p m ----
-#pragma unroll
-      for (int n = 0; n < kSets; ++n) {
-        l[0] += p[n][0] + p[n][2];
-        l[1] += p[n][1] + p[n][3];
+        // ---- O^T += V^T (p s)^T, z += p m ----
+        l[0] += p[0] + p[2];
+        l[1] += p[1] + p[3];
         const uint8_t* v_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4) + HB * S::kPageBytes;
         uint32_t vw[2][NG];
         kv4_params<NG>(v_par, vw[0]);
@@ -617,9 +602,9 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
             const int g = gp * 2 + j;
             const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
             const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
-            z[g][0] = fmaf(p[n][2], m1, fmaf(p[n][0], m0, z[g][0]));
-            z[g][1] = fmaf(p[n][3], m1, fmaf(p[n][1], m0, z[g][1]));
-            const float f[4] = {p[n][0] * s0, p[n][1] * s0, p[n][2] * s1, p[n][3] * s1};
+            z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
+            z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
+            const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
             const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
             pb[j][0] = movmatrix_trans(h0);
             pb[j][1] = movmatrix_trans(h1);
@@ -769,55 +754,58 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
 }
 
 // Merges the partials of the sequence that CTA blockIdx.x of the split kernel started and did not finish:
-// four warps a row, each over every fourth piece, lanes over values.
-template <typename T, int D>
+// WPR warps a row, each over every WPR-th piece, lanes over values.  One warp a row where sequences are
+// cut a few times (the chain of dependent loads is what costs: 3 us), eight where they are cut often.
+template <typename T, int D, int WPR>
 __global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4DecodeArgs a) {
-  constexpr int PER = D / 32, WPR = 4;
+  constexpr int PER = D / 32;
   using Vec = typename std::conditional<PER == 4, float4, float2>::type;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // programmatic dependent of the split kernel
   const Kv4Cut cut = a.cuts[blockIdx.x];
   if (cut.pieces == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.y * (8 / WPR) + warp / WPR;
   const int part = warp % WPR;
-  const bool live = row < a.part_rows;
-  // piece i: CTA blockIdx.x + i, in its first slot but for the first piece
-  const int64_t first = ((int64_t)blockIdx.x * 2 + cut.slot) * a.part_rows + (live ? row : 0);
-  const int64_t second = ((int64_t)blockIdx.x * 2 + 2) * a.part_rows + (live ? row : 0);
-  auto at = [&](int i) { return i == 0 ? first : second + (int64_t)(i - 1) * 2 * a.part_rows; };
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
-  float m_all = -INFINITY;
-  for (int i = lane; i < cut.pieces; i += 32) m_all = fmaxf(m_all, ml[at(i)].x);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, off));
-  float acc[PER], l = 0.f;
-#pragma unroll
-  for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int i = part; i < cut.pieces; i += WPR) {
-    const float2 x = ml[at(i)];
-    const Vec v = *reinterpret_cast<const Vec*>(a.ws_o + at(i) * D + lane * PER);
-    const float f = m_all == -INFINITY ? 1.f : ex2_approx(x.x - m_all);
-    l = fmaf(f, x.y, l);
-#pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], acc[e]);
-  }
   __shared__ float sa[8][D + 1];
+  for (int row = blockIdx.y * (8 / WPR) + warp / WPR; row < a.part_rows; row += gridDim.y * (8 / WPR)) {
+    // piece i: CTA blockIdx.x + i, in its first slot but for the first piece
+    const int64_t first = ((int64_t)blockIdx.x * 2 + cut.slot) * a.part_rows + row;
+    const int64_t second = ((int64_t)blockIdx.x * 2 + 2) * a.part_rows + row;
+    auto at = [&](int i) { return i == 0 ? first : second + (int64_t)(i - 1) * 2 * a.part_rows; };
+    float m_all = -INFINITY;
+    for (int i = lane; i < cut.pieces; i += 32) m_all = fmaxf(m_all, ml[at(i)].x);
 #pragma unroll
-  for (int e = 0; e < PER; ++e) sa[warp][lane * PER + e] = acc[e];
-  if (lane == 0) sa[warp][D] = l;
-  __syncthreads();
-  if (part != 0 || !live) return;
+    for (int off = 16; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, off));
+    float acc[PER], l = 0.f;
 #pragma unroll
-  for (int i = 1; i < WPR; ++i) {
+    for (int i = 0; i < PER; ++i) acc[i] = 0.f;
+#pragma unroll 4
+    for (int i = part; i < cut.pieces; i += WPR) {
+      const float2 x = ml[at(i)];
+      const Vec v = *reinterpret_cast<const Vec*>(a.ws_o + at(i) * D + lane * PER);
+      const float f = m_all == -INFINITY ? 1.f : ex2_approx(x.x - m_all);
+      l = fmaf(f, x.y, l);
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] += sa[warp + i][lane * PER + e];
-    l += sa[warp + i][D];
+      for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], acc[e]);
+    }
+    if constexpr (WPR > 1) {  // one row a CTA: the loop runs once
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sa[warp][lane * PER + e] = acc[e];
+      if (lane == 0) sa[warp][D] = l;
+      __syncthreads();
+      if (part != 0) return;
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] += sa[warp + i][lane * PER + e];
+        l += sa[warp + i][D];
+      }
+    }
+    T* dst = reinterpret_cast<T*>(a.out + cut.b * a.out_sb) + ((int64_t)cut.hb * a.part_rows + row) * D + lane * PER;
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
   }
-  T* dst = reinterpret_cast<T*>(a.out + cut.b * a.out_sb) + ((int64_t)cut.hb * a.part_rows + row) * D + lane * PER;
-  const float inv = 1.f / l;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) dst[e] = Elem<T>::from_f(acc[e] * inv);
 }
 
 template <typename T, int D, int BS, int HB, int SH>
@@ -838,10 +826,13 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
   cfg.numAttrs = 1;
   e = cudaLaunchKernelEx(&cfg, kern, a);
   if (e != cudaSuccess || a.whole) return e;
-  cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)((a.part_rows + 1) / 2));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D>, a);
+  if (a.ctas > 16 * a.batch * (a.hkv / HB)) {
+    cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)a.part_rows);
+    return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 8>, a);
+  }
+  return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 1>, a);
 }
 
 template <typename T, int D, int BS>
