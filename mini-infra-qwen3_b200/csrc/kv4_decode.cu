@@ -326,35 +326,39 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
     // ---------------- producer: lane 2p + kv copies K or V of page p of a step ----------------
     constexpr uint32_t kBytes = HB * S::kPageBytes;
     const int my_page = lane >> 1;
-    const bool mine = my_page < PG;
     const char* pool = (lane & 1) ? a.v_pool : a.k_pool;
     const int64_t block_bytes = (int64_t)a.hkv * S::kPageBytes;
-    const int64_t* table = a.block_tables + w.b * a.table_stride;
-    int n_pages = (w.ctx + BS - 1) / BS;
-    int64_t next_blk = 0;  // each lane reads its block id one step ahead, across sequences too
-    if (mine && w.pos * PG + my_page < n_pages) next_blk = table[w.pos * PG + my_page];
+    // Block ids come 32 pages at a time, one a lane, the next 32 (of the next sequence at the end of one)
+    // loaded while these are used.
+    static_assert(32 % PG == 0, "a step's pages lie in one window");
+    auto ids_from = [&](int64_t b, int page) {
+      return page + lane < a.max_blocks ? a.block_tables[b * a.table_stride + page + lane] : 0;
+    };
+    int64_t ids_next = ids_from(w.b, w.pos * PG);
     while (true) {
       const int n = w.take();
       const bool more = w.rest > n;
-      const bool next_row = (w.hb + 1) == nhb;
-      const int next_ctx = more ? (next_row ? kv4_ctx(a, w.b + 1) : w.ctx) : 0;
-      const int64_t* next_table = table + (next_row ? a.table_stride : 0);
+      const int64_t next_b = w.b + (w.hb + 1 == nhb);
+      const int next_ctx = more ? (next_b != w.b ? kv4_ctx(a, next_b) : w.ctx) : 0;
+      const int n_pages = (w.ctx + BS - 1) / BS;
       const int64_t head_off = (int64_t)w.hb * kBytes;
+      int64_t ids = 0;
       for (int s = 0; s < n; ++s) {
         const int first = (w.pos + s) * PG;
         const int npg = min(PG, n_pages - first);
-        int64_t blk = next_blk;
-        if (s + 1 < n) {
-          if (mine && first + PG + my_page < n_pages) next_blk = table[first + PG + my_page];
-        } else if (more) {
-          if (mine && my_page * BS < next_ctx) next_blk = next_table[my_page];
+        const int in = s * PG % 32;
+        if (in == 0) {
+          ids = ids_next;
+          if (s * PG + 32 < n * PG) ids_next = ids_from(w.b, first + 32);
+          else if (more) ids_next = ids_from(next_b, 0);
         }
+        int64_t blk = __shfl_sync(0xffffffffu, ids, in + (my_page < PG ? my_page : 0));
         if (npg <= 0) continue;  // a sequence of no tokens
         mbar_wait(&empty_bar[st], phase ^ 1, aborted);
         aborted = __any_sync(0xffffffffu, aborted);
         if (lane == 0) mbar_arrive_expect_tx(&full_bar[st], (uint32_t)npg * 2 * kBytes);
         __syncwarp();
-        if (mine && my_page < npg) {
+        if (my_page < npg) {
           if (blk < 0 || blk >= a.num_blocks) {
             record_status(MI_STATUS_BAD_BLOCK);
             blk = 0;  // the null block
@@ -366,8 +370,6 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
       }
       if (!more) return;
       kv4_advance<S::kTokens>(a, w, HB, next_ctx);
-      table = a.block_tables + w.b * a.table_stride;
-      n_pages = (w.ctx + BS - 1) / BS;
     }
   }
 
@@ -391,14 +393,29 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
   // ALU pipe, where the codes are cut, is the busiest.
   const __half2 ones[2] = {__float2half2_rn(r < 4 ? 1.f : 0.f), __float2half2_rn(r < 4 ? 0.f : 1.f)};
 
-  for (int64_t done = 0;; ) {  // one sequence's share at a time; `done`: steps of this CTA before it
-  const int n_steps = w.take();
-  const bool more = w.rest > n_steps;
-  const int next_ctx = more ? (w.hb + 1 == nhb ? kv4_ctx(a, w.b + 1) : w.ctx) : 0;
-  const int64_t b = w.b;
-  const int head0 = w.hb * HB;
-  const int h = head0 + hl;
-  int left = min(w.ctx - w.pos * S::kTokens, n_steps * S::kTokens) - un * kKv4Unit;  // tokens from this unit on
+  // What a warp knows of its place is kept in shared memory: the loop over the tokens needs the registers.
+  struct Place {
+    Kv4Walk w;
+    int64_t quota, done;  // done: steps of this CTA before the current sequence
+    int next_ctx;
+  };
+  __shared__ Place s_place[kKv4Consumers];
+  volatile Place& pl = s_place[warp];
+  if (lane == 0) {
+    Place first;
+    first.w = w;
+    first.quota = quota;
+    first.done = 0;
+    first.next_ctx = 0;
+    s_place[warp] = first;
+  }
+  __syncwarp();
+
+  while (true) {  // one sequence's share at a time
+  const int n_steps = (int)min(pl.w.rest, (int64_t)(pl.w.steps - pl.w.pos));
+  const int ctx = pl.w.ctx;
+  if (lane == 0 && pl.w.rest > n_steps) pl.next_ctx = pl.w.hb + 1 == nhb ? kv4_ctx(a, pl.w.b + 1) : ctx;
+  int left = min(ctx - pl.w.pos * S::kTokens, n_steps * S::kTokens) - un * kKv4Unit;  // tokens from this unit on
 
   // q as the B operand of S^T: this lane holds column r's values d = 32 g + 8 t + 0..7 of every group.
   // Column c is query head c % kCols; with SH = 2 the first four columns are for the first tile's
@@ -410,7 +427,8 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
     float qv[NG][8], qsum[NG];
     const bool valid = r % kCols < a.groups;
     const T* qp =
-        reinterpret_cast<const T*>(a.q + b * a.q_sb + (int64_t)(h * a.groups + (valid ? r % kCols : 0)) * a.q_sh);
+        reinterpret_cast<const T*>(a.q + pl.w.b * a.q_sb +
+                                   (int64_t)((pl.w.hb * HB + hl) * a.groups + (valid ? r % kCols : 0)) * a.q_sh);
     float top = 0.f;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
@@ -471,7 +489,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
 #pragma unroll
   for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
 
-  for (int it = w.ctx > 0 ? n_steps : 0; it > 0; --it, left -= S::kTokens) {
+  for (int it = ctx > 0 ? n_steps : 0; it > 0; --it, left -= S::kTokens) {
     mbar_wait(&full_bar[st], phase, aborted);
     if (left > 0) {
       const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
@@ -686,17 +704,21 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
   }
   auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
   // The rows' outputs where all of the sequence was here, else a partial: slot 0 the CTA's first, 1 its last.
-  const int slot = w.pos == 0 && n_steps == w.steps ? -1 : done > 0;
-  if (slot >= 0 && w.pos == 0 && threadIdx.x == 0) {  // the sequence starts here and is cut: say how often
+  const int64_t b = pl.w.b;
+  const int hb = pl.w.hb, pos = pl.w.pos, steps = pl.w.steps;
+  const int taken = (int)min(pl.w.rest, (int64_t)(steps - pos));
+  const int head0 = hb * HB;
+  const int slot = pos == 0 && taken == steps ? -1 : pl.done > 0;
+  if (slot >= 0 && pos == 0 && threadIdx.x == 0) {  // the sequence starts here and is cut: say how often
     Kv4Cut cut;
     cut.b = b;
-    cut.hb = w.hb;
+    cut.hb = hb;
     cut.slot = slot;
-    const int64_t at = blockIdx.x * quota + done;
-    cut.pieces = (int)((at + w.steps - 1) / quota - blockIdx.x) + 1;
+    const int64_t at = blockIdx.x * pl.quota + pl.done;
+    cut.pieces = (int)((at + steps - 1) / pl.quota - blockIdx.x) + 1;
     a.cuts[blockIdx.x] = cut;
   }
-  if (w.ctx == 0) {  // a row of no tokens
+  if (pl.w.ctx == 0) {  // a row of no tokens
     for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4Consumers * 32)
       reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
   } else if constexpr (UN > 1) {
@@ -742,14 +764,26 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
 #pragma unroll
       for (int g = 0; g < NG; ++g) {
         const float v[4] = {value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3)};
-        kv4_emit<T, D>(a, b, h * a.groups + head, slot, hl * a.groups + head, g * kKv4Group + r * 4, v, ref[c], l[c],
+        kv4_emit<T, D>(a, b, (head0 + hl) * a.groups + head, slot, hl * a.groups + head, g * kKv4Group + r * 4, v, ref[c], l[c],
                        g == 0 && r == 0);
       }
     }
   }
-  if (!more) return;
-  done += n_steps;
-  kv4_advance<S::kTokens>(a, w, HB, next_ctx);
+  if (pl.w.rest <= taken) return;
+  __syncwarp();
+  if (lane == 0) {
+    pl.done = pl.done + taken;
+    pl.w.rest = pl.w.rest - taken;
+    pl.w.pos = 0;
+    const bool row_done = hb + 1 == nhb;
+    pl.w.hb = row_done ? 0 : hb + 1;
+    if (row_done) {
+      pl.w.b = b + 1;
+      pl.w.ctx = pl.next_ctx;
+      pl.w.steps = kv4_steps<S::kTokens>(pl.next_ctx);
+    }
+  }
+  __syncwarp();
   }
 }
 
@@ -766,39 +800,61 @@ __global__ void __launch_bounds__(256) kv4_combine_kernel(const Kv4DecodeArgs a)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = warp % WPR;
   const float2* ml = reinterpret_cast<const float2*>(a.ws_ml);
-  __shared__ float sa[8][D + 1];
+  __shared__ float sa[8][D + 2];
   for (int row = blockIdx.y * (8 / WPR) + warp / WPR; row < a.part_rows; row += gridDim.y * (8 / WPR)) {
     // piece i: CTA blockIdx.x + i, in its first slot but for the first piece
     const int64_t first = ((int64_t)blockIdx.x * 2 + cut.slot) * a.part_rows + row;
     const int64_t second = ((int64_t)blockIdx.x * 2 + 2) * a.part_rows + row;
     auto at = [&](int i) { return i == 0 ? first : second + (int64_t)(i - 1) * 2 * a.part_rows; };
-    float m_all = -INFINITY;
-    for (int i = lane; i < cut.pieces; i += 32) m_all = fmaxf(m_all, ml[at(i)].x);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, off));
-    float acc[PER], l = 0.f;
+    float m_all = -INFINITY, acc[PER], l = 0.f;
 #pragma unroll
     for (int i = 0; i < PER; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int i = part; i < cut.pieces; i += WPR) {
-      const float2 x = ml[at(i)];
-      const Vec v = *reinterpret_cast<const Vec*>(a.ws_o + at(i) * D + lane * PER);
-      const float f = m_all == -INFINITY ? 1.f : ex2_approx(x.x - m_all);
-      l = fmaf(f, x.y, l);
+    for (int i0 = part; i0 < cut.pieces; i0 += 4 * WPR) {  // four pieces' loads at once, then their sums
+      float2 x[4];
+      Vec v[4];
+      float m_new = m_all;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, reinterpret_cast<const float*>(&v)[e], acc[e]);
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + k * WPR;
+        x[k] = i < cut.pieces ? ml[at(i)] : make_float2(-INFINITY, 0.f);
+        v[k] = i < cut.pieces ? *reinterpret_cast<const Vec*>(a.ws_o + at(i) * D + lane * PER) : Vec{};
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m_new = fmaxf(m_new, x[k].x);
+      const float keep = m_new == -INFINITY ? 1.f : ex2_approx(m_all - m_new);
+      m_all = m_new;
+      l *= keep;
+#pragma unroll
+      for (int e = 0; e < PER; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float f = m_new == -INFINITY ? 1.f : ex2_approx(x[k].x - m_new);
+        l = fmaf(f, x[k].y, l);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, reinterpret_cast<const float*>(&v[k])[e], acc[e]);
+      }
     }
     if constexpr (WPR > 1) {  // one row a CTA: the loop runs once
 #pragma unroll
       for (int e = 0; e < PER; ++e) sa[warp][lane * PER + e] = acc[e];
-      if (lane == 0) sa[warp][D] = l;
+      if (lane == 0) {
+        sa[warp][D] = l;
+        sa[warp][D + 1] = m_all;
+      }
       __syncthreads();
       if (part != 0) return;
+      m_all = sa[0][D + 1];
 #pragma unroll
-      for (int i = 1; i < WPR; ++i) {
+      for (int i = 1; i < WPR; ++i) m_all = fmaxf(m_all, sa[i][D + 1]);
+      l = 0.f;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) acc[e] += sa[warp + i][lane * PER + e];
-        l += sa[warp + i][D];
+      for (int e = 0; e < PER; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < WPR; ++i) {
+        const float f = m_all == -INFINITY ? 1.f : ex2_approx(sa[i][D + 1] - m_all);
+        l = fmaf(f, sa[i][D], l);
+#pragma unroll
+        for (int e = 0; e < PER; ++e) acc[e] = fmaf(f, sa[i][lane * PER + e], acc[e]);
       }
     }
     T* dst = reinterpret_cast<T*>(a.out + cut.b * a.out_sb) + ((int64_t)cut.hb * a.part_rows + row) * D + lane * PER;
@@ -832,6 +888,7 @@ cudaError_t launch_kv4_split(const Kv4DecodeArgs& a, cudaStream_t s) {
     cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)a.part_rows);
     return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 8>, a);
   }
+  cfg.gridDim = dim3((unsigned)a.ctas, (unsigned)((a.part_rows + 7) / 8));
   return cudaLaunchKernelEx(&cfg, kv4_combine_kernel<T, D, 1>, a);
 }
 
