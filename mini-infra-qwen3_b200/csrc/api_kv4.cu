@@ -17,6 +17,9 @@ int check_kv4_geometry(int64_t num_blocks, int block_size, int num_kv_heads, int
     return fail(MI_ERR_INVALID, "a 4-bit cache needs head_dim a multiple of %d up to 256 (got %d)", MI_KV4_GROUP,
                 head_dim);
   if (!aligned(k_pool, 4) || !aligned(v_pool, 4)) return fail(MI_ERR_INVALID, "4-bit pools must be 4-byte aligned");
+  if (num_blocks > kMaxGrid / block_size)
+    return fail(MI_ERR_UNSUPPORTED, "a pool of more than 2^31 - 1 tokens (%lld blocks of %d)", (long long)num_blocks,
+                block_size);
   return MI_OK;
 }
 
@@ -63,6 +66,7 @@ int mi_kv4_scatter(const void* k_src, const void* v_src, const int64_t* k_stride
   if (int rc = check_kv4_geometry(num_blocks, block_size, num_kv_heads, head_dim, dtype, k_pool, v_pool)) return rc;
   if (num_tokens < 0) return fail(MI_ERR_INVALID, "num_tokens < 0");
   if (num_tokens == 0) return MI_OK;
+  if (num_tokens > kMaxGrid) return fail(MI_ERR_UNSUPPORTED, "%lld tokens exceed one launch", (long long)num_tokens);
   if (!k_src || !v_src || !k_strides || !v_strides || !slot_mapping || !k_pool || !v_pool)
     return fail(MI_ERR_INVALID, "mi_kv4_scatter: null pointer argument");
   mi::Kv4StoreArgs a{};
@@ -90,6 +94,9 @@ int mi_kv4_store_chunks(const void* k_src, const void* v_src, const int64_t* k_s
   if (!k_src || !v_src || !k_strides || !v_strides || !chunk_lens || !start_positions || !block_tables || !k_pool ||
       !v_pool)
     return fail(MI_ERR_INVALID, "mi_kv4_store_chunks: null pointer argument");
+  if (padded_len > kMaxGrid / batch || table_width > kMaxGrid / block_size)
+    return fail(MI_ERR_UNSUPPORTED, "%lld x %lld positions or %lld blocks a row exceed one launch", (long long)batch,
+                (long long)padded_len, (long long)table_width);
   if (batch > 1 && table_stride < table_width)
     return fail(MI_ERR_INVALID, "block table rows of %lld entries at stride %lld", (long long)table_width,
                 (long long)table_stride);

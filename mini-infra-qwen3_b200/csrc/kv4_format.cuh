@@ -28,14 +28,18 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
 
 // Quantise a group spread over four consecutive lanes (eight values each): this lane's eight codes,
 // packed, and the group's parameter word.  `quad` is the mask of the four lanes.
+//
+// The code is the exact quotient (x - m) / s rounded to nearest even.  An IEEE division per value would
+// bound the store (90 us of a 20,000-token store against 17 us of traffic); a product with 1 / s is off
+// by at most 15 * 2^-23, so only a quotient that lands within 2^-17 of a tie is decided by its residual
+// (x - m) - c s, which one fma gives exactly.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned quad, uint32_t& word) {
-  float lo = x[0], hi = x[0];
-  bool finite = fabsf(x[0]) <= 3.402823466e38f;
+  float lo = x[0], hi = x[0], poison = 0.f;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) {
+  for (int i = 0; i < 8; ++i) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
-    finite = finite && fabsf(x[i]) <= 3.402823466e38f;  // false for NaN too
+    poison = fmaf(x[i], 0.f, poison);  // NaN from an infinity or a NaN
   }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
@@ -47,20 +51,43 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned q
   const uint32_t sb = bf16_bits(__fdiv_rn(hi - m, 15.f));
   const float s = __uint_as_float(sb << 16);
   // A group that no finite (s, m) describes reads back as NaN.
-  if (!__all_sync(quad, finite) || (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
+  if (!__all_sync(quad, poison == 0.f) || (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
     word = 0x7fc00000u;
     return 0u;
   }
   // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
   word = (mb << 16) | (s > 0.f ? sb : 0u);
   if (!(s > 0.f)) return 0u;
-  uint32_t code = 0;
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, nearest even
+  const bool normal = s >= 0x1p-126f && s <= 0x1p125f;
+  const float inv = normal ? __frcp_rn(s) : 0.f;
+  float c[8], worst = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(__fdiv_rn(x[i] - m, s)), 0.f), 15.f);
-    code |= (uint32_t)c << (4 * i);
+    const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
+    c[i] = (y + kRound) - kRound;
+    worst = fmaxf(worst, fabsf(y - c[i]));
   }
-  return code;
+  if (worst > 0.5f - 0x1p-17f || !normal) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float d = x[i] - m;
+      if (normal) {
+        const float e = fmaf(-c[i], s, d);  // residual against half a step; at a tie the even code
+        const float half = 0.5f * s;
+        const bool odd = ((int)c[i] & 1) != 0;
+        if (e > half || (e == half && odd)) c[i] += 1.f;
+        else if (e < -half || (e == -half && odd)) c[i] -= 1.f;
+      } else {
+        c[i] = rintf(__fdiv_rn(d, s));
+      }
+      c[i] = fminf(fmaxf(c[i], 0.f), 15.f);
+    }
+  }
+  // four codes are the digits of a 16-bit integer, read out of a float's mantissa
+  const float w0 = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))) + 8388608.f;
+  const float w1 = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4]))) + 8388608.f;
+  return __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
 }
 
 }  // namespace mi

@@ -1,7 +1,7 @@
 // Store and gather of the 4-bit paged cache (format: kv4_format.cuh).
 //
-// * kv4_scatter_kernel / kv4_store_chunks_kernel — quantise tokens into their slots, K and V in one
-//   launch; a thread takes eight values of K and the same eight of V, four lanes a group;
+// * kv4_store_kernel — quantises tokens into their slots, K and V in one launch: tokens at given slots or
+//   right-aligned chunks through block tables;
 // * kv4_gather_kernel — pages back as dense blocks in the model's type: out = T(m + s * c).
 #include <algorithm>
 
@@ -32,134 +32,139 @@ __device__ __forceinline__ void kv4_load8(const char* p, float (&x)[8]) {
   }
 }
 
-// Unit u (eight values of head h = u / (D/8)) of one token into slot (block, offset).
-template <typename T, bool VEC>
-__device__ __forceinline__ void kv4_put(const Kv4StoreArgs& a, const char* k_row, const char* v_row, int64_t block,
-                                        int offset, int u) {
-  const int per_head = a.head_dim >> 3;
-  const int h = u / per_head;
-  const int w = u - h * per_head;  // 8-value unit of the head; group w / 4
-  float k[8], v[8];
-  kv4_load8<T, VEC>(k_row + h * a.k_sb[1] + (int64_t)w * 8 * (int)sizeof(T), k);
-  kv4_load8<T, VEC>(v_row + h * a.v_sb[1] + (int64_t)w * 8 * (int)sizeof(T), v);
-  const unsigned quad = 0xfu << (threadIdx.x & 28);
-  uint32_t kw, vw;
-  const uint32_t kc = kv4_quantise(k, quad, kw);
-  const uint32_t vc = kv4_quantise(v, quad, vw);
-  const int64_t page = (block * a.heads + h) * a.page_bytes;
-  const int64_t code_at = page + ((int64_t)(w >> 2) * a.block_size + offset) * 16 + (w & 3) * 4;
-  *reinterpret_cast<uint32_t*>(a.k_pool + code_at) = kc;
-  *reinterpret_cast<uint32_t*>(a.v_pool + code_at) = vc;
-  if ((w & 3) == 0) {
-    const int64_t par_at = page + (int64_t)a.block_size * (a.head_dim >> 1) +
-                           ((int64_t)offset * (a.head_dim / kKv4Group) + (w >> 2)) * 4;
-    *reinterpret_cast<uint32_t*>(a.k_pool + par_at) = kw;
-    *reinterpret_cast<uint32_t*>(a.v_pool + par_at) = vw;
-  }
-}
-
-// Flat over (token, unit); the four lanes of a group always take the same path.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kKv4Threads) kv4_scatter_kernel(const Kv4StoreArgs a) {
-  const int units = a.heads * (a.head_dim >> 3);
-  const int64_t total = a.num_tokens * units;
-  for (int64_t i = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kKv4Threads) {
-    const int64_t token = i / units;
-    const int u = (int)(i - token * units);
+// A CTA takes eight tokens (a quad of lanes each: its slot is looked up once) and strides its warps over
+// the (head, group) pairs, a lane quantising eight values of K and the same eight of V.  A warp's eight
+// tokens of one group read 64-byte runs and, where the tokens share a page, write 128 contiguous bytes.
+template <typename T, bool VEC, bool CHUNKS>
+__global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5;
+  const unsigned quad = 0xfu << (lane & 28);
+  const unsigned tokens = (unsigned)(CHUNKS ? a.batch * a.padded_len : a.num_tokens);  // < 2^31
+  const unsigned token = blockIdx.x * 8u + (lane >> 2);
+  const bool tell = warp == 0 && blockIdx.y == 0 && (lane & 3) == 0;
+  if (token >= tokens) return;  // the four lanes of a token always take the same path
+  int64_t block, src_k, src_v;
+  unsigned offset;
+  if constexpr (CHUNKS) {
+    const unsigned row = token / (unsigned)a.padded_len;
+    const int64_t p = token - row * (unsigned)a.padded_len;
+    const int64_t first = a.padded_len - a.chunk_lens[row];
+    if (first < 0 && p == 0 && tell) record_status(MI_STATUS_BAD_LENGTH);  // only the last padded_len exist
+    if (p < first) return;
+    const int64_t pos = a.starts[row] + (p - first);
+    if (pos < 0 || pos >= a.table_width * a.block_size) {
+      if (tell) record_status(MI_STATUS_BAD_LENGTH);
+      return;
+    }
+    const unsigned logical = (unsigned)pos / (unsigned)a.block_size;  // pos < 2^31
+    offset = (unsigned)pos - logical * (unsigned)a.block_size;
+    block = a.block_tables[row * a.table_stride + logical];
+    if (block < 0 || block >= a.num_blocks) {
+      if (tell) record_status(MI_STATUS_BAD_BLOCK);
+      return;
+    }
+    src_k = row * a.k_sb[0] + p * a.k_sb[2];
+    src_v = row * a.v_sb[0] + p * a.v_sb[2];
+  } else {
     const int64_t slot = a.slots[token];
     if (slot < 0 || slot >= a.num_blocks * a.block_size) {
-      if (u == 0) record_status(MI_STATUS_BAD_SLOT);
-      continue;
+      if (tell) record_status(MI_STATUS_BAD_SLOT);
+      return;
     }
     const int64_t row = a.rows ? a.rows[token] : token;
     const int64_t pos = a.positions ? a.positions[token] : 0;
     if (row < 0 || row >= a.src_rows || pos < 0 || pos >= a.src_positions) {
-      if (u == 0) record_status(MI_STATUS_BAD_INDEX);
-      continue;
+      if (tell) record_status(MI_STATUS_BAD_INDEX);
+      return;
     }
-    const int64_t block = slot / a.block_size;
-    kv4_put<T, VEC>(a, a.k_src + row * a.k_sb[0] + pos * a.k_sb[2], a.v_src + row * a.v_sb[0] + pos * a.v_sb[2], block,
-                    (int)(slot - block * a.block_size), u);
+    block = (unsigned)slot / (unsigned)a.block_size;  // slots < 2^31
+    offset = (unsigned)slot - (unsigned)block * (unsigned)a.block_size;
+    src_k = row * a.k_sb[0] + pos * a.k_sb[2];
+    src_v = row * a.v_sb[0] + pos * a.v_sb[2];
+  }
+  const int ng = a.head_dim / kKv4Group;
+  const int w = lane & 3;  // eight-value quarter of the group
+  const int64_t page0 = block * a.heads * a.page_bytes;
+  const int64_t par0 = (int64_t)a.block_size * (a.head_dim >> 1) + (int64_t)offset * ng * 4;
+  const int pairs = a.heads * ng;
+  for (int pair = blockIdx.y * (kKv4Threads / 32) + warp; pair < pairs; pair += gridDim.y * (kKv4Threads / 32)) {
+    const int h = pair / ng;
+    const int g = pair - h * ng;
+    const int64_t at = (int64_t)(g * kKv4Group + w * 8) * (int)sizeof(T);
+    float k[8], v[8];
+    kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at, k);
+    kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at, v);
+    uint32_t kw, vw;
+    const uint32_t kc = kv4_quantise(k, quad, kw);
+    const uint32_t vc = kv4_quantise(v, quad, vw);
+    const int64_t page = page0 + h * a.page_bytes;
+    const int64_t code_at = page + ((int64_t)g * a.block_size + offset) * 16 + w * 4;
+    *reinterpret_cast<uint32_t*>(a.k_pool + code_at) = kc;
+    *reinterpret_cast<uint32_t*>(a.v_pool + code_at) = vc;
+    if (w == 0) {
+      *reinterpret_cast<uint32_t*>(a.k_pool + page + par0 + g * 4) = kw;
+      *reinterpret_cast<uint32_t*>(a.v_pool + page + par0 + g * 4) = vw;
+    }
   }
 }
 
-// Flat over (row, padded position, unit); padding positions are skipped.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kKv4Threads) kv4_store_chunks_kernel(const Kv4StoreArgs a) {
-  const int units = a.heads * (a.head_dim >> 3);
-  const int64_t total = a.batch * a.padded_len * units;
-  for (int64_t i = (int64_t)blockIdx.x * kKv4Threads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kKv4Threads) {
-    const int64_t item = i / units;  // row * padded_len + p
-    const int u = (int)(i - item * units);
-    const int64_t row = item / a.padded_len;
-    const int64_t p = item - row * a.padded_len;
-    const int64_t len = a.chunk_lens[row];
-    const int64_t first = a.padded_len - len;
-    if (first < 0 && p == 0 && u == 0) record_status(MI_STATUS_BAD_LENGTH);  // only the last padded_len exist
-    if (p < first) continue;
-    const int64_t pos = a.starts[row] + (p - first);
-    const int64_t logical = pos / a.block_size;
-    if (pos < 0 || logical >= a.table_width) {
-      if (u == 0) record_status(MI_STATUS_BAD_LENGTH);
-      continue;
-    }
-    const int64_t block = a.block_tables[row * a.table_stride + logical];
-    if (block < 0 || block >= a.num_blocks) {
-      if (u == 0) record_status(MI_STATUS_BAD_BLOCK);
-      continue;
-    }
-    kv4_put<T, VEC>(a, a.k_src + row * a.k_sb[0] + p * a.k_sb[2], a.v_src + row * a.v_sb[0] + p * a.v_sb[2], block,
-                    (int)(pos - logical * a.block_size), u);
-  }
-}
-
-// One CTA per gathered block: flat over (token, head, 8-value unit) of K, then of V.
-template <typename T>
+// One CTA per gathered block of K (blockIdx.y 0) or V (1): flat over (token, head, 8-value unit), a lane
+// reading four bytes of codes and writing eight values, so that a warp's stores are contiguous.  PH: units
+// of a head (head_dim / 8), 0 for one not known at compile time.
+template <typename T, int PH>
 __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4GatherArgs a) {
   constexpr int N = 16 / (int)sizeof(T);
-  const int64_t item = blockIdx.x;  // b * blocks_per_row + j
-  const int64_t b = item / a.blocks_per_row;
-  const int64_t j = item - b * a.blocks_per_row;
-  const int per_head = a.head_dim >> 3;
-  const int units = a.heads * per_head;  // per token
-  const int total = a.block_size * units;
+  constexpr int MLP = 4;  // units in flight a lane
+  const unsigned item = blockIdx.x;  // b * blocks_per_row + j
+  const unsigned b = item / (unsigned)a.blocks_per_row;
+  const int64_t j = item - b * (unsigned)a.blocks_per_row;
+  const int per_head = PH ? PH : a.head_dim >> 3;
+  const int rows = a.block_size * a.heads;  // (token, head)
+  const int total = rows * per_head;
   int64_t valid = a.block_size;  // tokens of this block that are read
   if (a.lengths) valid = min((int64_t)a.block_size, max((int64_t)0, a.lengths[b] - j * a.block_size));
   int64_t block = 0;
   if (valid > 0) {
     block = a.block_ids[b * a.id_stride + j];
     if (block < 0 || block >= a.num_blocks) {
-      if (threadIdx.x == 0) record_status(MI_STATUS_BAD_BLOCK);
+      if (threadIdx.x == 0 && blockIdx.y == 0) record_status(MI_STATUS_BAD_BLOCK);
       valid = 0;
     }
   }
   const int ng = a.head_dim / kKv4Group;
+  const char* pool = (blockIdx.y ? a.v_pool : a.k_pool) + block * a.heads * a.page_bytes;
+  const int par_off = a.block_size * (a.head_dim >> 1);
+  uint4* out = reinterpret_cast<uint4*>((blockIdx.y ? a.v_out : a.k_out) + (int64_t)item * total * 8 * (int)sizeof(T));
+  for (int i0 = threadIdx.x; i0 < total; i0 += MLP * kKv4Threads) {
+    uint32_t code[MLP], par[MLP];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const char* pool = kv ? a.v_pool : a.k_pool;
-    T* out = reinterpret_cast<T*>(kv ? a.v_out : a.k_out) + item * total * 8;
-    for (int i = threadIdx.x; i < total; i += kKv4Threads) {
-      const int t = i / units;
-      const int u = i - t * units;
-      const int h = u / per_head;
-      const int w = u - h * per_head;
+    for (int n = 0; n < MLP; ++n) {
+      const int i = i0 + n * kKv4Threads;
+      const int row = i / per_head, w = i - row * per_head;
+      const int t = row / a.heads, h = row - t * a.heads;
+      code[n] = par[n] = 0u;  // stands for zeros
+      if (i < total && t < valid) {
+        const char* page = pool + h * a.page_bytes;
+        code[n] = __ldg(reinterpret_cast<const uint32_t*>(page + ((w >> 2) * a.block_size + t) * 16) + (w & 3));
+        par[n] = __ldg(reinterpret_cast<const uint32_t*>(page + par_off) + t * ng + (w >> 2));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < MLP; ++n) {
+      const int i = i0 + n * kKv4Threads;
+      if (i >= total) break;
+      const float s = kv4_step(par[n]), m = kv4_min(par[n]);
       uint4 pk[8 / N];
       T* e = reinterpret_cast<T*>(pk);
-      if (t < valid) {
-        const char* page = pool + (block * a.heads + h) * a.page_bytes;
-        const uint32_t code =
-            __ldg(reinterpret_cast<const uint32_t*>(page + ((int64_t)(w >> 2) * a.block_size + t) * 16) + (w & 3));
-        const uint32_t par = __ldg(
-            reinterpret_cast<const uint32_t*>(page + (int64_t)a.block_size * (a.head_dim >> 1)) + t * ng + (w >> 2));
-        const float s = kv4_step(par), m = kv4_min(par);
 #pragma unroll
-        for (int n = 0; n < 8; ++n) e[n] = Elem<T>::from_f(fmaf((float)((code >> (4 * n)) & 15u), s, m));
-      } else {
-#pragma unroll
-        for (int n = 0; n < 8; ++n) e[n] = Elem<T>::from_f(0.f);
+      for (int c = 0; c < 8; ++c) {
+        // the code as the low mantissa bits of 2^23 + c
+        const float q = __uint_as_float(0x4b000000u | ((code[n] >> (4 * c)) & 15u)) - 8388608.f;
+        e[c] = Elem<T>::from_f(fmaf(q, s, m));
       }
 #pragma unroll
-      for (int n = 0; n < 8 / N; ++n) reinterpret_cast<uint4*>(out + (int64_t)i * 8)[n] = pk[n];
+      for (int c = 0; c < 8 / N; ++c) out[(int64_t)i * (8 / N) + c] = pk[c];
     }
   }
 }
@@ -167,15 +172,26 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
 template <typename T>
 cudaError_t launch_kv4_store_t(const Kv4StoreArgs& a, bool chunks, bool vec, cudaStream_t s) {
   const int64_t tokens = chunks ? a.batch * a.padded_len : a.num_tokens;
-  const int64_t threads = tokens * a.heads * (a.head_dim >> 3);
-  const unsigned grid = (unsigned)std::min<int64_t>((threads + kKv4Threads - 1) / kKv4Threads, 148 * 16);
+  const int64_t tiles = (tokens + 7) / 8;
+  const int pair_tiles = (a.heads * (a.head_dim / kKv4Group) + 7) / 8;
+  // every pair of a token in one CTA where the tokens fill the SMs, else the pairs spread over CTAs
+  const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 148 * 8 ? 1 : pair_tiles));
   if (chunks) {
-    if (vec) kv4_store_chunks_kernel<T, true><<<grid, kKv4Threads, 0, s>>>(a);
-    else kv4_store_chunks_kernel<T, false><<<grid, kKv4Threads, 0, s>>>(a);
+    if (vec) kv4_store_kernel<T, true, true><<<grid, kKv4Threads, 0, s>>>(a);
+    else kv4_store_kernel<T, false, true><<<grid, kKv4Threads, 0, s>>>(a);
   } else {
-    if (vec) kv4_scatter_kernel<T, true><<<grid, kKv4Threads, 0, s>>>(a);
-    else kv4_scatter_kernel<T, false><<<grid, kKv4Threads, 0, s>>>(a);
+    if (vec) kv4_store_kernel<T, true, false><<<grid, kKv4Threads, 0, s>>>(a);
+    else kv4_store_kernel<T, false, false><<<grid, kKv4Threads, 0, s>>>(a);
   }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_kv4_gather_t(const Kv4GatherArgs& a, cudaStream_t s) {
+  const dim3 grid((unsigned)(a.batch * a.blocks_per_row), 2);
+  if (a.head_dim == 128) kv4_gather_kernel<T, 16><<<grid, kKv4Threads, 0, s>>>(a);
+  else if (a.head_dim == 64) kv4_gather_kernel<T, 8><<<grid, kKv4Threads, 0, s>>>(a);
+  else kv4_gather_kernel<T, 0><<<grid, kKv4Threads, 0, s>>>(a);
   return cudaGetLastError();
 }
 
@@ -188,11 +204,9 @@ cudaError_t launch_kv4_store(const Kv4StoreArgs& a, bool chunks, bool vec, int d
 }
 
 cudaError_t launch_kv4_gather(const Kv4GatherArgs& a, int dtype, cudaStream_t s) {
-  const unsigned grid = (unsigned)(a.batch * a.blocks_per_row);
-  if (dtype == MI_BF16) kv4_gather_kernel<__nv_bfloat16><<<grid, kKv4Threads, 0, s>>>(a);
-  else if (dtype == MI_F16) kv4_gather_kernel<__half><<<grid, kKv4Threads, 0, s>>>(a);
-  else kv4_gather_kernel<float><<<grid, kKv4Threads, 0, s>>>(a);
-  return cudaGetLastError();
+  if (dtype == MI_BF16) return launch_kv4_gather_t<__nv_bfloat16>(a, s);
+  if (dtype == MI_F16) return launch_kv4_gather_t<__half>(a, s);
+  return launch_kv4_gather_t<float>(a, s);
 }
 
 }  // namespace mi
