@@ -7,6 +7,8 @@
 // transposed one whose rows are head_dim values (V), with no shuffle and no bank conflict.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mi {
@@ -26,68 +28,118 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
   return *reinterpret_cast<const uint16_t*>(&b);
 }
 
+// Eight consecutive values as they are in memory.
+template <typename T> struct Raw8 {
+  uint32_t w[8 * sizeof(T) / 4];
+  __device__ __forceinline__ float at(int i) const { return Elem<T>::to_f(reinterpret_cast<const T*>(w)[i]); }
+};
+
+// Smallest and largest of a group spread over the four lanes of `quad`; NaN where there is one.
+template <typename T>
+__device__ __forceinline__ void kv4_range(const Raw8<T>& x, unsigned quad, float& lo, float& hi) {
+  if constexpr (sizeof(T) == 2) {
+    // two values an instruction; (lo, -hi) as one pair that a minimum reduces
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* p = reinterpret_cast<const T2*>(x.w);
+    const T2 least = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
+    const T2 most = __hneg2(__hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3])));
+    const uint32_t a = *reinterpret_cast<const uint32_t*>(&least), b = *reinterpret_cast<const uint32_t*>(&most);
+    const uint32_t low = __byte_perm(a, b, 0x5410), high = __byte_perm(a, b, 0x7632);
+    T2 both = __hmin2_nan(*reinterpret_cast<const T2*>(&low), *reinterpret_cast<const T2*>(&high));
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const uint32_t other = __shfl_xor_sync(quad, *reinterpret_cast<const uint32_t*>(&both), o);
+      both = __hmin2_nan(both, *reinterpret_cast<const T2*>(&other));
+    }
+    lo = Elem<T>::to_f(both.x);
+    hi = -Elem<T>::to_f(both.y);
+  } else {
+    lo = hi = x.at(0);
+    float poison = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      lo = fminf(lo, x.at(i));
+      hi = fmaxf(hi, x.at(i));
+      poison = fmaf(x.at(i), 0.f, poison);  // NaN from a NaN (or an infinity)
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
+      poison += __shfl_xor_sync(quad, poison, o);
+    }
+    lo += poison;
+  }
+}
+
 // Quantise a group spread over four consecutive lanes (eight values each): this lane's eight codes,
 // packed, and the group's parameter word.  `quad` is the mask of the four lanes.
 //
-// The code is the exact quotient (x - m) / s rounded to nearest even.  An IEEE division per value would
-// bound the store (90 us of a 20,000-token store against 17 us of traffic); a product with 1 / s is off
-// by at most 15 * 2^-23, so only a quotient that lands within 2^-17 of a tie is decided by its residual
-// (x - m) - c s, which one fma gives exactly.
-__device__ __forceinline__ uint32_t kv4_quantise(const float (&x)[8], unsigned quad, uint32_t& word) {
-  float lo = x[0], hi = x[0], poison = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-    poison = fmaf(x[i], 0.f, poison);  // NaN from an infinity or a NaN
-  }
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
-  }
+// An IEEE division per value would bound the store (90 us of a 20,000-token store against 17 us of
+// traffic).  The quotient is (x - m) * (1 / s) instead, off by at most 15.5 * 1.5 * 2^-23 < 2^-18, and
+// ties, which 16-bit values meet every few hundred, are kept exact by rounding it to a multiple of 2^-17
+// first: a quotient within 2^-18 of half way counts as half way (and goes to the even code).
+template <typename T>
+__device__ __forceinline__ uint32_t kv4_quantise(const Raw8<T>& x, unsigned quad, uint32_t& word) {
+  float lo, hi;
+  kv4_range<T>(x, quad, lo, hi);
   const uint32_t mb = bf16_bits(lo);
   const float m = __uint_as_float(mb << 16);
   const uint32_t sb = bf16_bits(__fdiv_rn(hi - m, 15.f));
   const float s = __uint_as_float(sb << 16);
-  // A group that no finite (s, m) describes reads back as NaN.
-  if (!__all_sync(quad, poison == 0.f) || (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
+  // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s).
+  if ((mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
     word = 0x7fc00000u;
     return 0u;
   }
   // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
   word = (mb << 16) | (s > 0.f ? sb : 0u);
   if (!(s > 0.f)) return 0u;
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, nearest even
-  const bool normal = s >= 0x1p-126f && s <= 0x1p125f;
-  const float inv = normal ? __frcp_rn(s) : 0.f;
-  float c[8], worst = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = fminf(fmaxf((x[i] - m) * inv, 0.f), 15.f);
-    c[i] = (y + kRound) - kRound;
-    worst = fmaxf(worst, fabsf(y - c[i]));
-  }
-  if (worst > 0.5f - 0x1p-17f || !normal) {
+  float c[8];
+  if (s >= 0x1p-120f && s <= 0x1p120f) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within 2^-23
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float d = x[i] - m;
-      if (normal) {
-        const float e = fmaf(-c[i], s, d);  // residual against half a step; at a tie the even code
-        const float half = 0.5f * s;
-        const bool odd = ((int)c[i] & 1) != 0;
-        if (e > half || (e == half && odd)) c[i] += 1.f;
-        else if (e < -half || (e == -half && odd)) c[i] -= 1.f;
-      } else {
-        c[i] = rintf(__fdiv_rn(d, s));
-      }
-      c[i] = fminf(fmaxf(c[i], 0.f), 15.f);
+      const float y = fmaxf((x.at(i) - m) * inv, 0.f);  // at most 15 (1 + 2^-8): s is rounded too
+      c[i] = (((y + 96.f) - 96.f) + 12582912.f) - 12582912.f;  // to 2^-17, then to an integer
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(x.at(i) - m, s)), 0.f), 15.f);
   }
   // four codes are the digits of a 16-bit integer, read out of a float's mantissa
   const float w0 = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))) + 8388608.f;
   const float w1 = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4]))) + 8388608.f;
   return __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
+}
+
+// The eight values that packed codes and a parameter word stand for, rounded once to T.
+template <typename T>
+__device__ __forceinline__ Raw8<T> kv4_values(uint32_t code, uint32_t par) {
+  Raw8<T> v;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    // c as 128 + c in a bfloat16's mantissa, less 128; s c + m is one fused operation on the stored halves
+    const uint32_t s2 = __byte_perm(par, par, 0x1010), m2 = __byte_perm(par, par, 0x3232);
+    const uint32_t next = code >> 4;
+    const __nv_bfloat162 base = __float2bfloat162_rn(128.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // byte i of the word holds codes 2i and 2i + 1
+      const uint32_t pair = (__byte_perm(code, next, 0x0400 + 0x0101 * i) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&pair), base);
+      const __nv_bfloat162 r =
+          __hfma2(c, *reinterpret_cast<const __nv_bfloat162*>(&s2), *reinterpret_cast<const __nv_bfloat162*>(&m2));
+      v.w[i] = *reinterpret_cast<const uint32_t*>(&r);
+    }
+  } else {
+    const float s = kv4_step(par), m = kv4_min(par);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = __uint_as_float(0x4b000000u | ((code >> (4 * i)) & 15u)) - 8388608.f;  // 2^23 + c, less 2^23
+      reinterpret_cast<T*>(v.w)[i] = Elem<T>::from_f(fmaf(c, s, m));
+    }
+  }
+  return v;
 }
 
 }  // namespace mi

@@ -14,22 +14,19 @@ namespace {
 
 constexpr int kKv4Threads = 256;
 
-// Eight consecutive elements as floats; one or two 16-byte loads when the host proved them aligned.
+// Eight consecutive elements; 16-byte loads when the host proved them aligned.
 template <typename T, bool VEC>
-__device__ __forceinline__ void kv4_load8(const char* p, float (&x)[8]) {
+__device__ __forceinline__ Raw8<T> kv4_load8(const char* p) {
+  Raw8<T> x;
   if constexpr (VEC) {
-    constexpr int N = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 8 / N; ++j) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + j);
-      const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int i = 0; i < N; ++i) x[j * N + i] = Elem<T>::to_f(e[i]);
-    }
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+      reinterpret_cast<uint4*>(x.w)[j] = __ldg(reinterpret_cast<const uint4*>(p) + j);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f(reinterpret_cast<const T*>(p)[i]);
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(x.w)[i] = reinterpret_cast<const T*>(p)[i];
   }
+  return x;
 }
 
 // A CTA takes eight tokens (a quad of lanes each: its slot is looked up once) and strides its warps over
@@ -92,12 +89,11 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreAr
     const int h = pair / ng;
     const int g = pair - h * ng;
     const int64_t at = (int64_t)(g * kKv4Group + w * 8) * (int)sizeof(T);
-    float k[8], v[8];
-    kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at, k);
-    kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at, v);
+    const Raw8<T> k = kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at);
+    const Raw8<T> v = kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at);
     uint32_t kw, vw;
-    const uint32_t kc = kv4_quantise(k, quad, kw);
-    const uint32_t vc = kv4_quantise(v, quad, vw);
+    const uint32_t kc = kv4_quantise<T>(k, quad, kw);
+    const uint32_t vc = kv4_quantise<T>(v, quad, vw);
     const int64_t page = page0 + h * a.page_bytes;
     const int64_t code_at = page + ((int64_t)g * a.block_size + offset) * 16 + w * 4;
     *reinterpret_cast<uint32_t*>(a.k_pool + code_at) = kc;
@@ -136,35 +132,38 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
   const char* pool = (blockIdx.y ? a.v_pool : a.k_pool) + block * a.heads * a.page_bytes;
   const int par_off = a.block_size * (a.head_dim >> 1);
   uint4* out = reinterpret_cast<uint4*>((blockIdx.y ? a.v_out : a.k_out) + (int64_t)item * total * 8 * (int)sizeof(T));
+  // Unit i is 8-value unit w of (token t, head h); stepping by a CTA's width moves the three by fixed amounts.
+  const int row0 = threadIdx.x / per_head;
+  int w = threadIdx.x - row0 * per_head;
+  int t = row0 / a.heads;
+  int h = row0 - t * a.heads;
+  const int step_row = kKv4Threads / per_head, step_w = kKv4Threads - step_row * per_head;
+  const int step_t = step_row / a.heads, step_h = step_row - step_t * a.heads;
   for (int i0 = threadIdx.x; i0 < total; i0 += MLP * kKv4Threads) {
     uint32_t code[MLP], par[MLP];
 #pragma unroll
     for (int n = 0; n < MLP; ++n) {
-      const int i = i0 + n * kKv4Threads;
-      const int row = i / per_head, w = i - row * per_head;
-      const int t = row / a.heads, h = row - t * a.heads;
       code[n] = par[n] = 0u;  // stands for zeros
-      if (i < total && t < valid) {
+      if (t < valid) {
         const char* page = pool + h * a.page_bytes;
         code[n] = __ldg(reinterpret_cast<const uint32_t*>(page + ((w >> 2) * a.block_size + t) * 16) + (w & 3));
         par[n] = __ldg(reinterpret_cast<const uint32_t*>(page + par_off) + t * ng + (w >> 2));
       }
+      t += step_t;
+      h += step_h;
+      if (!(PH && kKv4Threads % PH == 0)) {
+        w += step_w;
+        if (w >= per_head) w -= per_head, ++h;
+      }
+      if (h >= a.heads) h -= a.heads, ++t;
     }
 #pragma unroll
     for (int n = 0; n < MLP; ++n) {
       const int i = i0 + n * kKv4Threads;
       if (i >= total) break;
-      const float s = kv4_step(par[n]), m = kv4_min(par[n]);
-      uint4 pk[8 / N];
-      T* e = reinterpret_cast<T*>(pk);
+      const Raw8<T> v = kv4_values<T>(code[n], par[n]);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        // the code as the low mantissa bits of 2^23 + c
-        const float q = __uint_as_float(0x4b000000u | ((code[n] >> (4 * c)) & 15u)) - 8388608.f;
-        e[c] = Elem<T>::from_f(fmaf(q, s, m));
-      }
-#pragma unroll
-      for (int c = 0; c < 8 / N; ++c) out[(int64_t)i * (8 / N) + c] = pk[c];
+      for (int c = 0; c < 8 / N; ++c) out[(int64_t)i * (8 / N) + c] = reinterpret_cast<const uint4*>(v.w)[c];
     }
   }
 }
