@@ -8,8 +8,10 @@ per-device buffer that grows on demand (the library itself never allocates).
 
 from __future__ import annotations
 
-import contextlib
+import array
 import ctypes
+import itertools
+import operator
 from collections.abc import Sequence
 
 import torch
@@ -504,11 +506,22 @@ def decode_rows(
 KV4_GROUP = 32  # values along head_dim that share a step and a minimum
 
 
-def _on(device: torch.device):
-    """A context with `device` current (launches go to the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_A2, _A3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+_NBYTES = operator.attrgetter("nbytes")
+
+
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Call an entry point with the device's current stream as its last argument, that device being current
+    (launches go to the current device), and raise its error."""
+    fn = getattr(nat.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device.index)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream)
+    if rc:
+        nat.check(rc, name)
 
 
 def kv_copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
@@ -518,23 +531,26 @@ def kv_copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     type, 4-bit pages among them.  Destinations must be distinct and not be sources of other pairs
     (nothing orders the pairs; ``PagedKVCachePool.copy_blocks`` checks that); (b, b) does nothing.
     Ids out of range are skipped and set MI_STATUS_BAD_BLOCK."""
-    device = _require_cuda("kv_copy_blocks", pairs, *pools)
+    device = _require_cuda("kv_copy_blocks", pairs)
+    if pairs.dtype != torch.int64 or pairs.ndim != 2 or pairs.shape[1] != 2:
+        raise ValueError(f"pairs must be int64 [n, 2], got {tuple(pairs.shape)} {pairs.dtype}")
     if not pools:
         return
-    blocks, size = pools[0].shape[0] if pools[0].ndim else 0, pools[0].nbytes
-    for p in pools:
-        if p.ndim < 2 or p.shape[0] != blocks or p.nbytes != size or not p.is_contiguous():
-            raise ValueError("pools must be contiguous [num_blocks, ...] tensors of the same blocks and bytes")
-    pairs = _index(pairs, "pairs")
-    if pairs.ndim != 2 or pairs.shape[1] != 2:
-        raise ValueError(f"pairs must be [n, 2], got {tuple(pairs.shape)}")
+    # a pool per layer, K and V: C-level maps, a Python loop over them would cost more than the copy
+    first = pools[0]
+    size = first.nbytes
+    if set(map(torch.Tensor.get_device, pools)) != {device.index}:
+        _require_cuda("kv_copy_blocks", pairs, *pools)
+    if (first.ndim < 2 or set(map(_NBYTES, pools)) != {size} or not all(map(torch.Tensor.is_contiguous, pools))
+            or set(map(torch.Tensor.size, pools, itertools.repeat(0))) != {first.shape[0]}):
+        raise ValueError("pools must be contiguous [num_blocks, ...] tensors of the same blocks and bytes")
+    blocks = first.shape[0]
     if blocks == 0 or size == 0:
         return
-    table = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
-    with _on(device):
-        rc = nat.load().mi_kv_copy_blocks(table, len(pools), _ptr(pairs), pairs.shape[0], blocks, size // blocks,
-                                          _stream(device))
-    nat.check(rc, "mi_kv_copy_blocks")
+    if not pairs.is_contiguous():
+        pairs = pairs.contiguous()
+    table = array.array("Q", map(torch.Tensor.data_ptr, pools))
+    _launch(device, "mi_kv_copy_blocks", table.buffer_info()[0], len(pools), pairs.data_ptr(), pairs.shape[0], blocks, size // blocks)
 
 
 def kv4_page_bytes(block_size: int, head_dim: int) -> int:
@@ -547,15 +563,16 @@ def kv4_page_bytes(block_size: int, head_dim: int) -> int:
 
 def _check_kv4(k_pool: torch.Tensor, v_pool: torch.Tensor, head_dim: int) -> tuple[int, int, int]:
     """(num_blocks, block_size, num_kv_heads) of 4-bit pools for this head_dim."""
-    if (k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or k_pool.ndim != 3 or k_pool.shape != v_pool.shape
+    shape = k_pool.shape
+    if (k_pool.dtype != torch.uint8 or v_pool.dtype != torch.uint8 or len(shape) != 3 or shape != v_pool.shape
             or not k_pool.is_contiguous() or not v_pool.is_contiguous()):
         raise ValueError(f"4-bit pools must be contiguous uint8 [num_blocks, num_kv_heads, page bytes], got "
-                         f"{tuple(k_pool.shape)} {k_pool.dtype} / {tuple(v_pool.shape)} {v_pool.dtype}")
-    n, h, page = k_pool.shape
-    bs = page // kv4_page_bytes(1, head_dim)
-    if bs < 1 or bs * kv4_page_bytes(1, head_dim) != page:
+                         f"{tuple(shape)} {k_pool.dtype} / {tuple(v_pool.shape)} {v_pool.dtype}")
+    n, h, page = shape
+    token = kv4_page_bytes(1, head_dim)
+    if page < token or page % token:
         raise ValueError(f"pages of {page} bytes hold no whole number of tokens of head_dim {head_dim}")
-    return n, bs, h
+    return n, page // token, h
 
 
 def kv4_scatter(
@@ -593,12 +610,9 @@ def kv4_scatter(
             raise ValueError(f"{name} has {t.numel()} entries, slot_mapping {slots.numel()}")
     if rows is None and slots.numel() > key.shape[0]:
         raise ValueError(f"{slots.numel()} slots for a source of {key.shape[0]} rows")
-    with _on(device):
-        rc = nat.load().mi_kv4_scatter(
-            _ptr(key), _ptr(value), nat.i64_array(ks), nat.i64_array(vs), key.shape[0], src_positions, _ptr(rows),
-            _ptr(positions), _ptr(slots), slots.numel(), _ptr(k_pool), _ptr(v_pool), n, bs, h, d,
-            dtype_code(key.dtype), _stream(device))
-    nat.check(rc, "mi_kv4_scatter")
+    _launch(device, "mi_kv4_scatter", key.data_ptr(), value.data_ptr(), _A3(*ks), _A3(*vs), key.shape[0], src_positions,
+            rows.data_ptr() if rows is not None else None, positions.data_ptr() if positions is not None else None,
+            slots.data_ptr(), slots.numel(), k_pool.data_ptr(), v_pool.data_ptr(), n, bs, h, d, dtype_code(key.dtype))
 
 
 def kv4_store_chunks(
@@ -625,12 +639,9 @@ def kv4_store_chunks(
     starts = _index(start_positions, "start_positions")
     if lens.numel() != b or starts.numel() != b or tables.ndim != 2 or tables.shape[0] != b:
         raise ValueError("chunk_lens, start_positions and block_tables need one row per batch row")
-    with _on(device):
-        rc = nat.load().mi_kv4_store_chunks(
-            _ptr(key), _ptr(value), nat.i64_array(key.stride()[:3]), nat.i64_array(value.stride()[:3]), b, length,
-            _ptr(lens), _ptr(starts), _ptr(tables), tables.shape[1], tables.shape[1], _ptr(k_pool), _ptr(v_pool), n,
-            bs, h, d, dtype_code(key.dtype), _stream(device))
-    nat.check(rc, "mi_kv4_store_chunks")
+    _launch(device, "mi_kv4_store_chunks", key.data_ptr(), value.data_ptr(), _A3(*key.stride()[:3]),
+            _A3(*value.stride()[:3]), b, length, lens.data_ptr(), starts.data_ptr(), tables.data_ptr(), tables.shape[1],
+            tables.shape[1], k_pool.data_ptr(), v_pool.data_ptr(), n, bs, h, d, dtype_code(key.dtype))
 
 
 def kv4_gather_blocks(
@@ -657,11 +668,9 @@ def kv4_gather_blocks(
     code = dtype_code(dtype)
     key = torch.empty((b, nb, bs, h, head_dim), dtype=dtype, device=device)
     value = torch.empty_like(key)
-    with _on(device):
-        rc = nat.load().mi_kv4_gather_blocks(
-            _ptr(k_pool), _ptr(v_pool), _ptr(ids), ids.stride(0) if b > 1 else nb, _ptr(lengths), b, nb, _ptr(key),
-            _ptr(value), n, bs, h, head_dim, code, _stream(device))
-    nat.check(rc, "mi_kv4_gather_blocks")
+    _launch(device, "mi_kv4_gather_blocks", k_pool.data_ptr(), v_pool.data_ptr(), ids.data_ptr(),
+            ids.stride(0) if b > 1 else nb, lengths.data_ptr() if lengths is not None else None, b, nb, key.data_ptr(),
+            value.data_ptr(), n, bs, h, head_dim, code)
     return key, value
 
 
@@ -700,7 +709,7 @@ def kv4_paged_decode(
         raise ValueError(f"context_lens has {ctx.numel()} entries for batch {b}")
     if hq < 1 or hq % h:
         raise ValueError(f"{hq} query heads are not a multiple of {h} KV heads")
-    new_strides = None
+    new = (None, None, None, None)
     if (key_new is None) != (value_new is None) or (key_new is None) != (slot_mapping is None):
         raise ValueError("key_new, value_new and slot_mapping go together")
     if key_new is not None:
@@ -710,27 +719,22 @@ def kv4_paged_decode(
         key_new, value_new = _rows_contiguous_last(key_new), _rows_contiguous_last(value_new)
         if key_new.stride() != value_new.stride():
             key_new, value_new = key_new.contiguous(), value_new.contiguous()
-        new_strides = nat.i64_array(key_new.stride()[:2])
         slot_mapping = _index(slot_mapping, "slot_mapping")
+        new = (key_new.data_ptr(), value_new.data_ptr(), _A2(*key_new.stride()[:2]), slot_mapping.data_ptr())
     if out is None:
         out = torch.empty((b, hq * d), dtype=query.dtype, device=device)
     elif out.shape != (b, hq * d) or out.dtype != query.dtype or out.stride(-1) != 1:
         raise ValueError(f"out must be [{b}, {hq * d}] {query.dtype} with contiguous rows")
     if b == 0:
         return out
-    lib = nat.load()
-    need = int(lib.mi_kv4_paged_decode_workspace_size(b, hq, h, d, width, bs, code))
+    need = nat.load().mi_kv4_paged_decode_workspace_size(b, hq, h, d, width, bs, code)
     base, avail = None, 0
     if need:
         if ws is None:
             ws = torch.empty(need + 256, dtype=torch.uint8, device=device)
         base = (ws.data_ptr() + 255) & ~255
         avail = ws.nbytes - (base - ws.data_ptr())
-    with _on(device):
-        rc = lib.mi_kv4_paged_decode(
-            _ptr(query), nat.i64_array(query.stride()[:2]), _ptr(key_new), _ptr(value_new), new_strides,
-            _ptr(slot_mapping), _ptr(k_pool), _ptr(v_pool), n, bs, h, d, _ptr(tables),
-            tables.stride(0) if b > 1 else width, width, _ptr(ctx), b, hq, float(scale), _ptr(out), out.stride(0), base,
-            avail, code, _stream(device))
-    nat.check(rc, "mi_kv4_paged_decode")
+    _launch(device, "mi_kv4_paged_decode", query.data_ptr(), _A2(*query.stride()[:2]), *new,
+            k_pool.data_ptr(), v_pool.data_ptr(), n, bs, h, d, tables.data_ptr(), tables.stride(0) if b > 1 else width,
+            width, ctx.data_ptr(), b, hq, float(scale), out.data_ptr(), out.stride(0), base, avail, code)
     return out
