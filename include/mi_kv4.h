@@ -61,12 +61,14 @@ int mi_kv4_store_chunks(const void* k_src, const void* v_src, const int64_t* k_s
  * block_ids[b * id_stride + j], rounded to dtype; k_out/v_out contiguous
  * [batch, blocks_per_row, block_size, num_kv_heads, head_dim], the layout of a dense pool of
  * batch * blocks_per_row blocks.  With lengths (NULL: all), row b's tokens at and past lengths[b] are
- * written as zeros, whatever the pages hold there, and the ids of blocks wholly past it are not read.
- * A block id out of range reads as zeros and sets MI_STATUS_BAD_BLOCK.
+ * written as zeros, whatever the pages hold there, and the ids of blocks wholly past it are not read;
+ * with fill_past == 0 those blocks are not written either (the attention reads none of them).  A block id out of range reads as zeros and sets
+ * MI_STATUS_BAD_BLOCK.
  */
 int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* block_ids, int64_t id_stride,
-                         const int64_t* lengths, int64_t batch, int64_t blocks_per_row, void* k_out, void* v_out,
-                         int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int dtype, void* stream);
+                         const int64_t* lengths, int fill_past, int64_t batch, int64_t blocks_per_row, void* k_out,
+                         void* v_out, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int dtype,
+                         void* stream);
 
 /*
  * mi_kv4_paged_decode — mi_paged_decode over 4-bit pools: one query token per sequence attends to

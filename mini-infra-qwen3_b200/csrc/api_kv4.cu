@@ -116,8 +116,9 @@ int mi_kv4_store_chunks(const void* k_src, const void* v_src, const int64_t* k_s
 }
 
 int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* block_ids, int64_t id_stride,
-                         const int64_t* lengths, int64_t batch, int64_t blocks_per_row, void* k_out, void* v_out,
-                         int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int dtype, void* stream) {
+                         const int64_t* lengths, int fill_past, int64_t batch, int64_t blocks_per_row, void* k_out,
+                         void* v_out, int64_t num_blocks, int block_size, int num_kv_heads, int head_dim, int dtype,
+                         void* stream) {
   if (int rc = check_kv4_geometry(num_blocks, block_size, num_kv_heads, head_dim, dtype, k_pool, v_pool)) return rc;
   if (batch < 0 || blocks_per_row < 0) return fail(MI_ERR_INVALID, "negative size");
   if (batch == 0 || blocks_per_row == 0) return MI_OK;
@@ -138,6 +139,7 @@ int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* 
   a.block_ids = block_ids;
   a.id_stride = id_stride;
   a.lengths = lengths;
+  a.fill_past = fill_past;
   a.batch = batch;
   a.blocks_per_row = blocks_per_row;
   a.k_out = static_cast<char*>(k_out);

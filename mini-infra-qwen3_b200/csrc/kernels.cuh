@@ -253,6 +253,7 @@ struct Kv4GatherArgs {
   const int64_t* block_ids;
   int64_t id_stride;
   const int64_t* lengths;  // may be null: every token
+  int fill_past;           // write the blocks past a row's length (zeros)
   int64_t batch;
   int64_t blocks_per_row;
   char* k_out;

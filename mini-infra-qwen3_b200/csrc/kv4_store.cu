@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
   const int total = rows * per_head;
   int64_t valid = a.block_size;  // tokens of this block that are read
   if (a.lengths) valid = min((int64_t)a.block_size, max((int64_t)0, a.lengths[b] - j * a.block_size));
+  if (valid == 0 && !a.fill_past) return;
   int64_t block = 0;
   if (valid > 0) {
     block = a.block_ids[b * a.id_stride + j];
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
       }
       t += step_t;
       h += step_h;
-      if (!(PH && kKv4Threads % PH == 0)) {
+      if (PH == 0 || kKv4Threads % (PH ? PH : 1) != 0) {
         w += step_w;
         if (w >= per_head) w -= per_head, ++h;
       }

@@ -13,9 +13,14 @@ input depend on it:
   ``block_release_count`` and ``peak_used_blocks``.
 
 Design here: the free list is a fixed-capacity ring over the num_blocks - 1 allocatable ids (a
-block id is either in the ring or in exactly one table, so the ring never overflows); a bytearray
+block id is either in the ring or in some table, so the ring never overflows); a bytearray
 marks the ids handed out before; each request holds a lease of its table and cached token count;
 admission is a bisection over the prefix sums of the waiting prompts' block needs.
+
+Not in the reference: ``fork`` lets a second request continue from the first one's tokens, sharing its full
+blocks (counted, and freed by their last holder) and taking a copy of a partly filled last one;
+``compact`` renumbers the blocks in use into 1 .. num_used_blocks.  Both return the (src, dst) block copies
+that the pools have to make (``PagedKVCachePool.copy_blocks``) before the next step.
 """
 
 from __future__ import annotations
@@ -100,6 +105,17 @@ class FreeKVCacheBlockQueue:
             released += 1
         self.release_count += released
 
+    def exchange(self, moves: Sequence[tuple[int, int]]) -> None:
+        """For each (used, free) pair, the free id becomes used and the used one takes its place in the queue."""
+        freed = {d: s for s, d in moves}
+        cap = len(self._ring)
+        for i in range(self._free):
+            at = (self._head + i) % cap
+            if self._ring[at] in freed:
+                d = self._ring[at]
+                self._ring[at] = freed[d]
+                self._handed_out_before[d] = 1
+
 
 @dataclass
 class _Lease:
@@ -118,6 +134,7 @@ class KVCacheManager:
         self.block_size = block_size
         self.free_block_queue = FreeKVCacheBlockQueue(num_blocks)
         self._leases: dict[int, _Lease] = {}
+        self._sharers: dict[int, int] = {}  # blocks in several tables -> how many beyond the first
 
     @property
     def num_used_blocks(self) -> int:
@@ -166,8 +183,47 @@ class KVCacheManager:
         return True
 
     def free(self, request_idx: int) -> None:
-        """Release the request's blocks (KeyError for a request holding no lease)."""
-        self.free_block_queue.free(self._leases.pop(request_idx).table)
+        """Release the request's blocks (KeyError for a request holding no lease); a block that other
+        requests share stays theirs."""
+        own = []
+        for b in self._leases.pop(request_idx).table:
+            others = self._sharers.pop(b, 0)
+            if others > 1:
+                self._sharers[b] = others - 1
+            if others == 0:
+                own.append(b)
+        self.free_block_queue.free(own)
+
+    def fork(self, request_idx: int, new_request_idx: int) -> list[tuple[int, int]] | None:
+        """Give new_request_idx the request's cached tokens: its full blocks are shared, a partly filled
+        last one is copied to a block of its own.  Returns the copies to make, (src, dst), at most one;
+        None (and no change) when the block that takes is not free.  KeyError for a request holding no
+        lease, ValueError for a new request that holds one."""
+        lease = self._leases[request_idx]
+        if new_request_idx in self._leases:
+            raise ValueError(f"request {new_request_idx} already holds blocks")
+        full = lease.tokens // self.block_size
+        copied = lease.table[full:]
+        if len(copied) > self.free_block_queue.num_free_blocks:
+            return None
+        for b in lease.table[:full]:
+            self._sharers[b] = self._sharers.get(b, 0) + 1
+        new = self.free_block_queue.allocate(len(copied))
+        self._leases[new_request_idx] = _Lease(lease.table[:full] + new, lease.tokens)
+        return list(zip(copied, new))
+
+    def compact(self) -> list[tuple[int, int]]:
+        """Renumber the blocks in use into 1 .. num_used_blocks, moving as few as possible; every table
+        follows.  Returns the copies to make, (src, dst): no destination is a source."""
+        used = {b for lease in self._leases.values() for b in lease.table}
+        holes = [b for b in range(NULL_BLOCK_ID + 1, len(used) + 1) if b not in used]
+        moves = list(zip(sorted(b for b in used if b > len(used)), holes))
+        to = dict(moves)
+        for lease in self._leases.values():
+            lease.table[:] = [to.get(b, b) for b in lease.table]
+        self._sharers = {to.get(b, b): n for b, n in self._sharers.items()}
+        self.free_block_queue.exchange(moves)
+        return moves
 
 
 __all__ = ["FreeKVCacheBlockQueue", "KVCacheManager", "NULL_BLOCK_ID", "num_blocks_for_tokens", "required_pool_blocks"]

@@ -56,20 +56,27 @@ class DenseCacheConfig:
 @dataclass(frozen=True)
 class PagedCacheConfig:
     """Paged KV cache: tokens per block, and the pool size in blocks including the null block
-    (None = derived from the workload by ``required_pool_blocks``)."""
+    (None = derived from the workload by ``required_pool_blocks``).
+
+    ``kv_bits`` (no counterpart in the reference): 16 keeps K and V in the model's type; 4 in 4-bit
+    codes with a step and a minimum per 32 values (head_dim a multiple of 32 up to 256)."""
 
     kind: ClassVar[KVCacheKind] = "paged-kv-cache"
     block_size: int = 16
     num_blocks: int | None = None
+    kv_bits: int = 16
 
     def __post_init__(self) -> None:
         if self.block_size < 1:
             raise ValueError("block_size must be positive")
         if self.num_blocks is not None and self.num_blocks < 2:
             raise ValueError("num_blocks must be >= 2 (block 0 is the null block)")
+        if self.kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 (the model's type) or 4, got {self.kv_bits}")
 
     def __str__(self) -> str:
         extra = f",num_blocks={self.num_blocks}" if self.num_blocks is not None else ""
+        extra += f",kv_bits={self.kv_bits}" if self.kv_bits != 16 else ""
         return f"{self.kind}(block_size={self.block_size}{extra})"
 
 
@@ -77,14 +84,15 @@ KVCacheConfig = NoCacheConfig | DenseCacheConfig | PagedCacheConfig
 
 
 def kv_cache_config_from_str(
-    kind: str | None, *, block_size: int | None = None, num_blocks: int | None = None
+    kind: str | None, *, block_size: int | None = None, num_blocks: int | None = None, kv_bits: int | None = None
 ) -> KVCacheConfig:
     parsed = parse_kv_cache_kind(kind)
     if parsed == "none":
         return NoCacheConfig()
     if parsed == "dense-kv-cache":
         return DenseCacheConfig()
-    return PagedCacheConfig(block_size=16 if block_size is None else block_size, num_blocks=num_blocks)
+    return PagedCacheConfig(block_size=16 if block_size is None else block_size, num_blocks=num_blocks,
+                            kv_bits=16 if kv_bits is None else kv_bits)
 
 
 def _positive_budget(budget: int) -> None:

@@ -26,7 +26,7 @@ from mini_infra_b200.core.types import BatchingMethod, PagedCacheConfig
 from mini_infra_b200.device import synchronize
 from mini_infra_b200.engine.metrics import PagedCacheProfile
 from mini_infra_b200.engine.schedule_backend import ScheduleStepOutput
-from mini_infra_b200.worker import PagedKVCachePool, PagedRunner
+from mini_infra_b200.worker import PagedKV4CachePool, PagedKVCachePool, PagedRunner
 
 
 class PagedScheduleBackend:
@@ -60,7 +60,8 @@ class PagedScheduleBackend:
         config = model.config  # type: ignore[attr-defined]
         attn = model.model.layers[0].self_attn  # type: ignore[attr-defined]
         self.runner = PagedRunner(model, pad_token_id)
-        self.pool = PagedKVCachePool(
+        four_bit = paged_cache_config.kv_bits == 4
+        self.pool = (PagedKV4CachePool if four_bit else PagedKVCachePool)(
             num_layers=config.num_hidden_layers,
             num_blocks=num_blocks,
             block_size=self.block_size,
@@ -85,7 +86,7 @@ class PagedScheduleBackend:
             if current is not None and (not peer_exchange or current.max_rows < rows):
                 detach_peer_exchange(model)
                 current = None
-            if peer_exchange and current is None:
+            if peer_exchange and current is None and not four_bit:  # a 4-bit decode is followed by NCCL's
                 attach_peer_exchange(model, rows, self.block_size)
         if cuda_graphs and self.device.type == "cuda":
             # decode tables never exceed the largest request; round the graphs' width up to a power of two
@@ -97,6 +98,14 @@ class PagedScheduleBackend:
         """Drop the decode and mixed-step graphs (they may hold NCCL calls: before the process group goes)."""
         self.runner.release_decode_graphs()
         self.runner.release_mixed_graphs()
+
+    def compact(self) -> int:
+        """Move the blocks in use to the lowest ids (between steps); returns how many moved."""
+        moves = self.kv_cache_manager.compact()
+        self.pool.copy_blocks(moves)
+        if self.runner.device_tables is not None:
+            self.runner.device_tables.invalidate()
+        return len(moves)
 
     @property
     def kv_cache_config(self) -> PagedCacheConfig:

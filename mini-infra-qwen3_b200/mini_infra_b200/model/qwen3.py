@@ -24,6 +24,10 @@ Attention has two entry forms:
 Tensor layout inside the model: activations [B, L, hidden]; Q/K/V [B, L, heads, head_dim].
 Present K/V returned by prefill are [B, H_kv, L, D] views (the reference's ``KVCache`` layout).
 
+With 4-bit pools (uint8 pages, ``PagedKV4CachePool``) the same two forms run on ``mi_kv4_paged_decode``,
+after the store that quantises the new K/V, and on the dense gather of the history's blocks followed by
+``mi_paged_prefill``.
+
 Head partition (``tp_world > 1``): the layer keeps query heads [r*Hq/P, (r+1)*Hq/P) and KV heads
 [r*H/P, (r+1)*H/P); its pools hold only those KV heads; the attention output is all-gathered
 over the process group before the replicated o_proj — on decode, when a ``PeerExchange`` is
@@ -165,6 +169,11 @@ def gather_heads(attn: torch.Tensor, partition: HeadPartition) -> torch.Tensor:
     return gathered.view(partition.world, n, width).transpose(0, 1).reshape(n, partition.world * width)
 
 
+def _paged_prefill(key_pool: torch.Tensor | None):
+    """The chunked-prefill operator of a pool's kind (16- and 32-bit pools hold elements, 4-bit ones bytes)."""
+    return ops.kv4_paged_prefill if key_pool is not None and key_pool.dtype == torch.uint8 else ops.paged_prefill
+
+
 class Qwen3Attention(nn.Module):
     def __init__(self, config: Qwen3Config, partition: HeadPartition = HeadPartition()):
         super().__init__()
@@ -198,6 +207,10 @@ class Qwen3Attention(nn.Module):
         if isinstance(metadata, PagedAttentionMetadata):
             # decode: norm + RoPE, and the new K/V appended to the pools, in one launch
             key_pool, value_pool = kv_pool
+            if key_pool.dtype == torch.uint8:
+                attn = self._decode_kv4(q, k, v, cos2, sin2, kv_pool, metadata)
+                attn = gather_heads(attn, self.partition).view(b, length, -1)
+                return self.o_proj(attn), kv_pool
             q_out, _, _ = ops.qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos2, sin2, self.q_norm.eps,
                                            self.num_heads, self.num_kv_heads, kv_out=False,
                                            slot_mapping=metadata.slot_mapping, k_pool=key_pool, v_pool=value_pool)
@@ -216,7 +229,7 @@ class Qwen3Attention(nn.Module):
             k4 = k_out.view(b, length, self.num_kv_heads, d)
             v4 = v_out.view(b, length, self.num_kv_heads, d)
             key_pool, value_pool = kv_pool if kv_pool is not None else (None, None)
-            attn = ops.paged_prefill(
+            attn = _paged_prefill(key_pool)(
                 q_out.view(b, length, self.num_heads, d), k4, v4, key_pool, value_pool, metadata.block_tables,
                 metadata.start_positions, metadata.chunk_lens, self.scaling,
             )
@@ -224,13 +237,22 @@ class Qwen3Attention(nn.Module):
         attn = gather_heads(attn.view(tokens, -1), self.partition).view(b, length, -1)
         return self.o_proj(attn), present
 
+    def _decode_kv4(self, q, k, v, cos2, sin2, kv_pool: PastKeyValue, md: PagedAttentionMetadata, out=None):
+        """Decode rows over 4-bit pools: norm + RoPE, then the new K/V quantised into the pools and attended to."""
+        q_out, k_out, v_out = ops.qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos2, sin2,
+                                               self.q_norm.eps, self.num_heads, self.num_kv_heads)
+        return ops.kv4_paged_decode(q_out, *kv_pool, md.block_tables, md.context_lens, self.scaling, key_new=k_out,
+                                    value_new=v_out, slot_mapping=md.slot_mapping, out=out)
+
     def _mixed(self, q, k, v, cos2, sin2, kv_pool, md: "MixedMetadata", b: int, length: int):
         """Decode rows [0, nd) through the fused append + paged decode, chunk rows through the
         chunked-prefill kernel; both write into one attention buffer."""
         nd, bp, lp, d = md.num_decode, md.prefill_rows, md.prefill_len, self.head_dim
         key_pool, value_pool = kv_pool
         attn = torch.empty((nd + bp * lp, self.num_heads * d), dtype=q.dtype, device=q.device)
-        if nd:
+        if nd and key_pool.dtype == torch.uint8:
+            self._decode_kv4(q[:nd], k[:nd], v[:nd], cos2[:nd], sin2[:nd], kv_pool, md.decode, out=attn[:nd])
+        elif nd:
             q_d, _, _ = ops.qk_norm_rope(q[:nd], k[:nd], v[:nd], self.q_norm.weight, self.k_norm.weight, cos2[:nd],
                                          sin2[:nd], self.q_norm.eps, self.num_heads, self.num_kv_heads, kv_out=False,
                                          slot_mapping=md.decode.slot_mapping, k_pool=key_pool, v_pool=value_pool)
@@ -240,9 +262,9 @@ class Qwen3Attention(nn.Module):
                                          sin2[nd:], self.q_norm.eps, self.num_heads, self.num_kv_heads)
         k4 = k_p.view(bp, lp, self.num_kv_heads, d)
         v4 = v_p.view(bp, lp, self.num_kv_heads, d)
-        ops.paged_prefill(q_p.view(bp, lp, self.num_heads, d), k4, v4, key_pool, value_pool, md.prefill.block_tables,
-                          md.prefill.start_positions, md.prefill.chunk_lens, self.scaling,
-                          out=attn[nd:].view(bp, lp, -1))
+        _paged_prefill(key_pool)(q_p.view(bp, lp, self.num_heads, d), k4, v4, key_pool, value_pool, md.prefill.block_tables,
+                                 md.prefill.start_positions, md.prefill.chunk_lens, self.scaling,
+                                 out=attn[nd:].view(bp, lp, -1))
         attn = gather_heads(attn, self.partition).view(b, length, -1)
         return self.o_proj(attn), (k4.transpose(1, 2), v4.transpose(1, 2))
 

@@ -184,6 +184,8 @@ def gather_blocks(pool: torch.Tensor, block_ids: torch.Tensor) -> torch.Tensor:
 
 
 def decode_workspace_bytes(batch: int, num_q_heads: int, k_pool: torch.Tensor, max_blocks: int) -> int:
+    if k_pool.dtype == torch.uint8:  # a 4-bit pool: kv4_paged_decode takes its workspace at the call
+        return 0
     n, bs, h, d = k_pool.shape
     return int(nat.load().mi_paged_decode_workspace_size(batch, num_q_heads, h, d, max_blocks, bs,
                                                          dtype_code(k_pool.dtype)))
@@ -651,10 +653,11 @@ def kv4_gather_blocks(
     head_dim: int,
     dtype: torch.dtype,
     lengths: torch.Tensor | None = None,
+    fill_past: bool = True,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """Blocks of 4-bit pools as dense ones: (key, value), each [B, nb, bs, H, D] in `dtype` for block_ids
     [B, nb].  With lengths [B], row b's tokens at and past lengths[b] are zeros and the ids of blocks past
-    it are not read."""
+    it are not read; fill_past=False leaves those blocks uninitialised."""
     device = _require_cuda("kv4_gather_blocks", k_pool, v_pool, block_ids, lengths)
     n, bs, h = _check_kv4(k_pool, v_pool, head_dim)
     if block_ids.dtype != torch.int64 or block_ids.ndim != 2:
@@ -669,7 +672,7 @@ def kv4_gather_blocks(
     key = torch.empty((b, nb, bs, h, head_dim), dtype=dtype, device=device)
     value = torch.empty_like(key)
     _launch(device, "mi_kv4_gather_blocks", k_pool.data_ptr(), v_pool.data_ptr(), ids.data_ptr(),
-            ids.stride(0) if b > 1 else nb, lengths.data_ptr() if lengths is not None else None, b, nb, key.data_ptr(),
+            ids.stride(0) if b > 1 else nb, lengths.data_ptr() if lengths is not None else None, int(fill_past), b, nb, key.data_ptr(),
             value.data_ptr(), n, bs, h, head_dim, code)
     return key, value
 
@@ -738,3 +741,29 @@ def kv4_paged_decode(
             k_pool.data_ptr(), v_pool.data_ptr(), n, bs, h, d, tables.data_ptr(), tables.stride(0) if b > 1 else width,
             width, ctx.data_ptr(), b, hq, float(scale), out.data_ptr(), out.stride(0), base, avail, code)
     return out
+
+
+def kv4_paged_prefill(
+    query: torch.Tensor,
+    key_chunk: torch.Tensor,
+    value_chunk: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+    block_tables: torch.Tensor,
+    start_positions: torch.Tensor,
+    chunk_lens: torch.Tensor,
+    scale: float,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``paged_prefill`` with its history in 4-bit pools: the history blocks are gathered as dense ones and
+    attended to; the chunk's own K/V enter as they are, unquantised."""
+    if block_tables.numel() == 0:
+        return paged_prefill(query, key_chunk, value_chunk, None, None, block_tables, start_positions, chunk_lens, scale,
+                             out=out)
+    d = query.shape[-1]
+    key, value = kv4_gather_blocks(k_pool, v_pool, block_tables, d, query.dtype, lengths=start_positions,
+                                   fill_past=False)
+    b, nb = block_tables.shape
+    dense = torch.arange(b * nb, device=query.device).view(b, nb)
+    return paged_prefill(query, key_chunk, value_chunk, key.flatten(0, 1), value.flatten(0, 1), dense, start_positions,
+                         chunk_lens, scale, out=out)

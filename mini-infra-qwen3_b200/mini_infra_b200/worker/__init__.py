@@ -2,7 +2,7 @@
 
 from mini_infra_b200.worker.base_runner import BaseModelRunner, PrefillOutput
 from mini_infra_b200.worker.kv_cache import KVCache, cache_size_bytes
-from mini_infra_b200.worker.paged_kv_cache import PagedKVCachePool
+from mini_infra_b200.worker.paged_kv_cache import PagedKV4CachePool, PagedKVCachePool
 from mini_infra_b200.worker.paged_runner import PagedDecodeOutput, PagedMixedOutput, PagedRunner
 from mini_infra_b200.worker.sampler import greedy_sample
 
@@ -11,6 +11,7 @@ __all__ = [
     "KVCache",
     "PagedDecodeOutput",
     "PagedMixedOutput",
+    "PagedKV4CachePool",
     "PagedKVCachePool",
     "PagedRunner",
     "PrefillOutput",

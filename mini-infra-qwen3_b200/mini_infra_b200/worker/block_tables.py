@@ -35,6 +35,11 @@ class DeviceBlockTables:
         self._synced = [0] * capacity  # entries of that table already on the device
         self._last = [0] * capacity  # the last of those entries (block id)
 
+    def invalidate(self) -> None:
+        """Forget what the rows hold (block ids changed under their sequences, as a compaction does): every
+        sequence's next step resends its table."""
+        self._owner = [None] * self.capacity
+
     def step_inputs(
         self,
         row_keys: Sequence[tuple[int, int]],
