@@ -343,6 +343,72 @@ def test_decode_matches_the_oracle(b, hq, h, d, bs, lengths, dtype):
     assert (err <= tol).all(), f"{(err / tol).max():.2f} of the tolerance"
 
 
+CUT = [
+    # batch, query heads, KV heads, head_dim, block size, longest, dtype: sequences cut over many CTAs, CTAs
+    # that hold many sequences, rows of no tokens between them
+    (1, 8, 1, 128, 16, 9000, "bf16"),
+    (1, 4, 2, 64, 32, 20011, "fp16"),
+    (2, 4, 4, 128, 16, 7001, "bf16"),
+    (300, 4, 1, 64, 16, 700, "bf16"),
+    (40, 8, 4, 128, 16, 1700, "fp16"),
+    (700, 2, 2, 64, 16, 90, "bf16"),     # short tables: whole sequences
+    (1000, 1, 1, 64, 16, 400, "bf16"),
+]
+
+
+@pytest.mark.parametrize("b,hq,h,d,bs,longest,dtype", CUT)
+def test_decode_of_streams_that_are_cut(b, hq, h, d, bs, longest, dtype):
+    rng = np.random.default_rng(b + longest)
+    ctx = np.minimum(rng.geometric(4 / longest, b), longest).astype(np.int64)
+    ctx[rng.integers(b)] = longest
+    if b > 2:
+        ctx[rng.integers(0, b, b // 8)] = 0
+        ctx[[0, -1]] = 0
+    # pages shared by all rows: what counts here is who takes which steps
+    blocks = 64
+    kp, vp = pools(rng, blocks, bs, h, d)
+    tables = rng.integers(1, blocks, (b, -(-longest // bs))).astype(np.int64)
+    q = tokens(rng, (b, hq, d), dtype)
+    scale = d**-0.5
+    got = ops.kv4_paged_decode(q, cuda(kp), cuda(vp), cuda(tables), cuda(ctx), scale)
+    assert ops.read_status() == 0
+    want = ko.decode(np64(q), kp, vp, tables, ctx, scale, bs)
+    tol = decode_tolerance(want, np64(q), kp, vp, tables, ctx, scale, bs, dtype)
+    err = np.abs(np64(got) - want)
+    assert (err <= tol).all(), f"{(err / tol).max():.2f} of the tolerance"
+    assert not got[torch.from_numpy(ctx == 0).cuda()].any()
+    again = ops.kv4_paged_decode(q, cuda(kp), cuda(vp), cuda(tables), cuda(ctx), scale)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("width", [3, 60])
+def test_bad_blocks_and_lengths_whole_or_cut(width):
+    """Flags and clamps on tables short enough for whole sequences and on longer ones, whose stream is cut."""
+    rng = np.random.default_rng(width)
+    b, hq, h, d, bs, blocks = 6, 8, 4, 128, 16, 20
+    kp, vp = (cuda(p) for p in pools(rng, blocks, bs, h, d))
+    q = tokens(rng, (b, hq, d), "bf16")
+    tables = rng.integers(1, blocks, (b, width)).astype(np.int64)
+    ctx = np.full(b, width * bs - 5, dtype=np.int64)
+    fine = ops.kv4_paged_decode(q, kp, vp, cuda(tables), cuda(ctx), 0.1)
+    bad, null = tables.copy(), tables.copy()
+    bad[1, 0], bad[3, width - 1], bad[4, 1] = -1, blocks, 1 << 60
+    null[1, 0] = null[3, width - 1] = null[4, 1] = 0
+    out = ops.kv4_paged_decode(q, kp, vp, cuda(bad), cuda(ctx), 0.1)
+    assert ops.read_status() == nat.MI_STATUS_BAD_BLOCK
+    assert torch.equal(out, ops.kv4_paged_decode(q, kp, vp, cuda(null), cuda(ctx), 0.1))
+    assert torch.equal(out[[0, 2, 5]], fine[[0, 2, 5]])
+    over = ctx.copy()
+    over[2], over[5] = width * bs + 1, 1 << 62
+    out = ops.kv4_paged_decode(q, kp, vp, cuda(tables), cuda(over), 0.1)
+    assert ops.read_status() == nat.MI_STATUS_BAD_LENGTH
+    over[[2, 5]] = width * bs
+    assert torch.equal(out, ops.kv4_paged_decode(q, kp, vp, cuda(tables), cuda(over), 0.1))
+    over[[0, 3]] = -(1 << 62)
+    out = ops.kv4_paged_decode(q, kp, vp, cuda(tables), cuda(over), 0.1)
+    assert not out[[0, 3]].any() and ops.read_status() == 0
+
+
 @pytest.mark.parametrize("d,bs,dtype", [(128, 16, "bf16"), (64, 32, "fp16"), (128, 32, "bf16"), (32, 5, "fp32")])
 def test_decode_at_every_length_of_a_page_and_none(d, bs, dtype):
     """Lengths 0 to two pages and one token in one batch, pages poisoned past every length: a row of none
