@@ -17,6 +17,8 @@ int check_kv4_geometry(int64_t num_blocks, int block_size, int num_kv_heads, int
     return fail(MI_ERR_INVALID, "a 4-bit cache needs head_dim a multiple of %d up to 256 (got %d)", MI_KV4_GROUP,
                 head_dim);
   if (!aligned(k_pool, 4) || !aligned(v_pool, 4)) return fail(MI_ERR_INVALID, "4-bit pools must be 4-byte aligned");
+  if (mi_kv4_page_bytes(block_size, head_dim) > kMaxGrid)
+    return fail(MI_ERR_UNSUPPORTED, "pages of more than 2^31 - 1 bytes");
   if (num_blocks > kMaxGrid / block_size)
     return fail(MI_ERR_UNSUPPORTED, "a pool of more than 2^31 - 1 tokens (%lld blocks of %d)", (long long)num_blocks,
                 block_size);

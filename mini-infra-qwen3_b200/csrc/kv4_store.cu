@@ -32,7 +32,8 @@ __device__ __forceinline__ Raw8<T> kv4_load8(const char* p) {
 // A CTA takes eight tokens (a quad of lanes each: its slot is looked up once) and strides its warps over
 // the (head, group) pairs, a lane quantising eight values of K and the same eight of V.  A warp's eight
 // tokens of one group read 64-byte runs and, where the tokens share a page, write 128 contiguous bytes.
-template <typename T, bool VEC, bool CHUNKS>
+// The next pair's loads are issued before this pair is quantised.  NG: groups of a head, 0 for any.
+template <typename T, bool VEC, bool CHUNKS, int NG>
 __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreArgs a) {
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
@@ -80,28 +81,44 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreAr
     src_k = row * a.k_sb[0] + pos * a.k_sb[2];
     src_v = row * a.v_sb[0] + pos * a.v_sb[2];
   }
-  const int ng = a.head_dim / kKv4Group;
+  const int ng = NG ? NG : a.head_dim / kKv4Group;
   const int w = lane & 3;  // eight-value quarter of the group
-  const int64_t page0 = block * a.heads * a.page_bytes;
-  const int64_t par0 = (int64_t)a.block_size * (a.head_dim >> 1) + (int64_t)offset * ng * 4;
+  char* k_page = a.k_pool + block * a.heads * a.page_bytes;
+  char* v_page = a.v_pool + block * a.heads * a.page_bytes;
+  const int par0 = a.block_size * (a.head_dim >> 1) + (int)offset * ng * 4;
   const int pairs = a.heads * ng;
-  for (int pair = blockIdx.y * (kKv4Threads / 32) + warp; pair < pairs; pair += gridDim.y * (kKv4Threads / 32)) {
+  const int step = gridDim.y * (kKv4Threads / 32);
+  auto load = [&](int pair, Raw8<T>& k, Raw8<T>& v) {
     const int h = pair / ng;
-    const int g = pair - h * ng;
-    const int64_t at = (int64_t)(g * kKv4Group + w * 8) * (int)sizeof(T);
-    const Raw8<T> k = kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at);
-    const Raw8<T> v = kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at);
+    const int at = ((pair - h * ng) * kKv4Group + w * 8) * (int)sizeof(T);
+    k = kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at);
+    v = kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at);
+  };
+  int pair = blockIdx.y * (kKv4Threads / 32) + warp;
+  if (pair >= pairs) return;
+  Raw8<T> k, v;
+  load(pair, k, v);
+  while (true) {
+    Raw8<T> k_next, v_next;
+    const bool more = pair + step < pairs;
+    if (more) load(pair + step, k_next, v_next);
     uint32_t kw, vw;
     const uint32_t kc = kv4_quantise<T>(k, quad, kw);
     const uint32_t vc = kv4_quantise<T>(v, quad, vw);
-    const int64_t page = page0 + h * a.page_bytes;
+    const int h = pair / ng;
+    const int g = pair - h * ng;
+    const int64_t page = h * a.page_bytes;
     const int64_t code_at = page + ((int64_t)g * a.block_size + offset) * 16 + w * 4;
-    *reinterpret_cast<uint32_t*>(a.k_pool + code_at) = kc;
-    *reinterpret_cast<uint32_t*>(a.v_pool + code_at) = vc;
+    *reinterpret_cast<uint32_t*>(k_page + code_at) = kc;
+    *reinterpret_cast<uint32_t*>(v_page + code_at) = vc;
     if (w == 0) {
-      *reinterpret_cast<uint32_t*>(a.k_pool + page + par0 + g * 4) = kw;
-      *reinterpret_cast<uint32_t*>(a.v_pool + page + par0 + g * 4) = vw;
+      *reinterpret_cast<uint32_t*>(k_page + page + par0 + g * 4) = kw;
+      *reinterpret_cast<uint32_t*>(v_page + page + par0 + g * 4) = vw;
     }
+    if (!more) return;
+    pair += step;
+    k = k_next;
+    v = v_next;
   }
 }
 
@@ -176,12 +193,16 @@ cudaError_t launch_kv4_store_t(const Kv4StoreArgs& a, bool chunks, bool vec, cud
   const int pair_tiles = (a.heads * (a.head_dim / kKv4Group) + 7) / 8;
   // every pair of a token in one CTA where the tokens fill the SMs, else the pairs spread over CTAs
   const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 148 * 8 ? 1 : pair_tiles));
+  auto launch = [&](auto kernel) { kernel<<<grid, kKv4Threads, 0, s>>>(a); };
+  const int ng = a.head_dim / kKv4Group;
   if (chunks) {
-    if (vec) kv4_store_kernel<T, true, true><<<grid, kKv4Threads, 0, s>>>(a);
-    else kv4_store_kernel<T, false, true><<<grid, kKv4Threads, 0, s>>>(a);
+    if (vec && ng == 4) launch(kv4_store_kernel<T, true, true, 4>);
+    else if (vec) launch(kv4_store_kernel<T, true, true, 0>);
+    else launch(kv4_store_kernel<T, false, true, 0>);
   } else {
-    if (vec) kv4_store_kernel<T, true, false><<<grid, kKv4Threads, 0, s>>>(a);
-    else kv4_store_kernel<T, false, false><<<grid, kKv4Threads, 0, s>>>(a);
+    if (vec && ng == 4) launch(kv4_store_kernel<T, true, false, 4>);
+    else if (vec) launch(kv4_store_kernel<T, true, false, 0>);
+    else launch(kv4_store_kernel<T, false, false, 0>);
   }
   return cudaGetLastError();
 }
