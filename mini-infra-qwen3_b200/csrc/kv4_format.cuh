@@ -32,6 +32,18 @@ __device__ __forceinline__ uint32_t bf16_bits(float x) {
 template <typename T> struct Raw8 {
   uint32_t w[8 * sizeof(T) / 4];
   __device__ __forceinline__ float at(int i) const { return Elem<T>::to_f(reinterpret_cast<const T*>(w)[i]); }
+  // value i less m, rounded to fp32: one instruction for the 16-bit types
+  __device__ __forceinline__ float less(int i, float m) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint16_t h = (uint16_t)(w[i >> 1] >> (16 * (i & 1)));
+      float d;
+      if constexpr (std::is_same<T, __half>::value) asm("sub.f32.f16 %0, %1, %2;" : "=f"(d) : "h"(h), "f"(m));
+      else asm("sub.f32.bf16 %0, %1, %2;" : "=f"(d) : "h"(h), "f"(m));
+      return d;
+    } else {
+      return at(i) - m;
+    }
+  }
 };
 
 // Smallest and largest of a group spread over the four lanes of `quad`; NaN where there is one.
@@ -72,22 +84,33 @@ __device__ __forceinline__ void kv4_range(const Raw8<T>& x, unsigned quad, float
   }
 }
 
+// x / 15, correctly rounded: one correction of the product with 1 / 15 (exact over all mantissas; tiny x,
+// whose residual would be subnormal, by division).
+__device__ __forceinline__ float div15(float x) {
+  if (fabsf(x) < 0x1p-100f) return __fdiv_rn(x, 15.f);
+  constexpr float r = 1.f / 15.f;
+  const float q = x * r;
+  return fmaf(fmaf(-15.f, q, x), r, q);
+}
+
 // Quantise a group spread over four consecutive lanes (eight values each): this lane's eight codes,
 // packed, and the group's parameter word.  `quad` is the mask of the four lanes.
 //
 // An IEEE division per value would bound the store (90 us of a 20,000-token store against 17 us of
 // traffic).  The quotient is (x - m) * (1 / s) instead, off by at most 15.5 * 1.5 * 2^-23 < 2^-18, and
 // ties, which 16-bit values meet every few hundred, are kept exact by rounding it to a multiple of 2^-17
-// first: a quotient within 2^-18 of half way counts as half way (and goes to the even code).
+// first: a quotient within 2^-18 of half way counts as half way (and goes to the even code).  Five
+// instructions a value: difference, product clamped to [0, 1) in units of 16, the two roundings, and the
+// code, the low bits of 1.5 * 2^23 + c, as a digit of the packed word.
 template <typename T>
 __device__ __forceinline__ uint32_t kv4_quantise(const Raw8<T>& x, unsigned quad, uint32_t& word) {
   float lo, hi;
   kv4_range<T>(x, quad, lo, hi);
   const uint32_t mb = bf16_bits(lo);
   const float m = __uint_as_float(mb << 16);
-  const uint32_t sb = bf16_bits(__fdiv_rn(hi - m, 15.f));
+  const uint32_t sb = bf16_bits(div15(hi - m));
   const float s = __uint_as_float(sb << 16);
-  // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s).
+  // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
   if ((mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
     word = 0x7fc00000u;
     return 0u;
@@ -95,23 +118,26 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Raw8<T>& x, unsigned quad
   // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
   word = (mb << 16) | (s > 0.f ? sb : 0u);
   if (!(s > 0.f)) return 0u;
-  float c[8];
-  if (s >= 0x1p-120f && s <= 0x1p120f) {
+  uint32_t code = 0;
+  if (s >= 0x1p-110f && s <= 0x1p110f) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within 2^-23
+    inv *= 0.0625f;
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to an integer
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float y = fmaxf((x.at(i) - m) * inv, 0.f);  // at most 15 (1 + 2^-8): s is rounded too
-      c[i] = (((y + 96.f) - 96.f) + 12582912.f) - 12582912.f;  // to 2^-17, then to an integer
+      const float y = __saturatef(x.less(i, m) * inv);    // a 16th of the quotient; at most 15 (1 + 2^-8) / 16
+      const float t = fmaf(y, 16.f, 96.f);                // the quotient to 2^-17
+      const uint32_t u = __float_as_uint(t + (kRound - 96.f));
+      code += u << (4 * i);  // 0x4b400000 + c
     }
+    code -= 0x4b400000u * 0x11111111u;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = fminf(fmaxf(rintf(__fdiv_rn(x.at(i) - m, s)), 0.f), 15.f);
+    for (int i = 0; i < 8; ++i)
+      code |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x.at(i) - m, s)), 0.f), 15.f) << (4 * i);
   }
-  // four codes are the digits of a 16-bit integer, read out of a float's mantissa
-  const float w0 = fmaf(c[3], 4096.f, fmaf(c[2], 256.f, fmaf(c[1], 16.f, c[0]))) + 8388608.f;
-  const float w1 = fmaf(c[7], 4096.f, fmaf(c[6], 256.f, fmaf(c[5], 16.f, c[4]))) + 8388608.f;
-  return __byte_perm(__float_as_uint(w0), __float_as_uint(w1), 0x5410);
+  return code;
 }
 
 // The eight values that packed codes and a parameter word stand for, rounded once to T.
