@@ -46,41 +46,41 @@ template <typename T> struct Raw8 {
   }
 };
 
-// Smallest and largest of a group spread over the four lanes of `quad`; NaN where there is one.
+// Smallest and largest of a group spread over the two lanes of `pair`; NaN where there is one.
 template <typename T>
-__device__ __forceinline__ void kv4_range(const Raw8<T>& x, unsigned quad, float& lo, float& hi) {
+__device__ __forceinline__ void kv4_range(const Raw8<T> (&x)[2], unsigned pair, float& lo, float& hi) {
   if constexpr (sizeof(T) == 2) {
     // two values an instruction; (lo, -hi) as one pair that a minimum reduces
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    const T2* p = reinterpret_cast<const T2*>(x.w);
-    const T2 least = __hmin2_nan(__hmin2_nan(p[0], p[1]), __hmin2_nan(p[2], p[3]));
-    const T2 most = __hneg2(__hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3])));
+    const T2* p = reinterpret_cast<const T2*>(x[0].w);
+    const T2* q = reinterpret_cast<const T2*>(x[1].w);
+    T2 least = __hmin2_nan(p[0], q[0]), most = __hmax2_nan(p[0], q[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      least = __hmin2_nan(least, __hmin2_nan(p[i], q[i]));
+      most = __hmax2_nan(most, __hmax2_nan(p[i], q[i]));
+    }
+    most = __hneg2(most);
     const uint32_t a = *reinterpret_cast<const uint32_t*>(&least), b = *reinterpret_cast<const uint32_t*>(&most);
     const uint32_t low = __byte_perm(a, b, 0x5410), high = __byte_perm(a, b, 0x7632);
     T2 both = __hmin2_nan(*reinterpret_cast<const T2*>(&low), *reinterpret_cast<const T2*>(&high));
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      const uint32_t other = __shfl_xor_sync(quad, *reinterpret_cast<const uint32_t*>(&both), o);
-      both = __hmin2_nan(both, *reinterpret_cast<const T2*>(&other));
-    }
+    const uint32_t other = __shfl_xor_sync(pair, *reinterpret_cast<const uint32_t*>(&both), 1);
+    both = __hmin2_nan(both, *reinterpret_cast<const T2*>(&other));
     lo = Elem<T>::to_f(both.x);
     hi = -Elem<T>::to_f(both.y);
   } else {
-    lo = hi = x.at(0);
+    lo = hi = x[0].at(0);
     float poison = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      lo = fminf(lo, x.at(i));
-      hi = fmaxf(hi, x.at(i));
-      poison = fmaf(x.at(i), 0.f, poison);  // NaN from a NaN (or an infinity)
+    for (int i = 0; i < 16; ++i) {
+      const float f = x[i >> 3].at(i & 7);
+      lo = fminf(lo, f);
+      hi = fmaxf(hi, f);
+      poison = fmaf(f, 0.f, poison);  // NaN from a NaN (or an infinity)
     }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
-      hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
-      poison += __shfl_xor_sync(quad, poison, o);
-    }
-    lo += poison;
+    lo = fminf(lo, __shfl_xor_sync(pair, lo, 1));
+    hi = fmaxf(hi, __shfl_xor_sync(pair, hi, 1));
+    lo += poison + __shfl_xor_sync(pair, poison, 1);
   }
 }
 
@@ -93,8 +93,8 @@ __device__ __forceinline__ float div15(float x) {
   return fmaf(fmaf(-15.f, q, x), r, q);
 }
 
-// Quantise a group spread over four consecutive lanes (eight values each): this lane's eight codes,
-// packed, and the group's parameter word.  `quad` is the mask of the four lanes.
+// Quantise a group spread over two consecutive lanes (twice eight values each): this lane's codes, eight a
+// word, and the group's parameter word.  `pair` is the mask of the two lanes.
 //
 // An IEEE division per value would bound the store (90 us of a 20,000-token store against 17 us of
 // traffic).  The quotient is (x - m) * (1 / s) instead, off by at most 15.5 * 1.5 * 2^-23 < 2^-18, and
@@ -103,9 +103,10 @@ __device__ __forceinline__ float div15(float x) {
 // instructions a value: difference, product clamped to [0, 1) in units of 16, the two roundings, and the
 // code, the low bits of 1.5 * 2^23 + c, as a digit of the packed word.
 template <typename T>
-__device__ __forceinline__ uint32_t kv4_quantise(const Raw8<T>& x, unsigned quad, uint32_t& word) {
+__device__ __forceinline__ void kv4_quantise(const Raw8<T> (&x)[2], unsigned pair, uint32_t (&code)[2], uint32_t& word) {
   float lo, hi;
-  kv4_range<T>(x, quad, lo, hi);
+  kv4_range<T>(x, pair, lo, hi);
+  code[0] = code[1] = 0u;
   const uint32_t mb = bf16_bits(lo);
   const float m = __uint_as_float(mb << 16);
   const uint32_t sb = bf16_bits(div15(hi - m));
@@ -113,31 +114,34 @@ __device__ __forceinline__ uint32_t kv4_quantise(const Raw8<T>& x, unsigned quad
   // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
   if ((mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
     word = 0x7fc00000u;
-    return 0u;
+    return;
   }
   // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
   word = (mb << 16) | (s > 0.f ? sb : 0u);
-  if (!(s > 0.f)) return 0u;
-  uint32_t code = 0;
+  if (!(s > 0.f)) return;
   if (s >= 0x1p-110f && s <= 0x1p110f) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within 2^-23
     inv *= 0.0625f;
     constexpr float kRound = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to an integer
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float y = __saturatef(x.less(i, m) * inv);    // a 16th of the quotient; at most 15 (1 + 2^-8) / 16
-      const float t = fmaf(y, 16.f, 96.f);                // the quotient to 2^-17
-      const uint32_t u = __float_as_uint(t + (kRound - 96.f));
-      code += u << (4 * i);  // 0x4b400000 + c
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __saturatef(x[n].less(i, m) * inv);  // a 16th of the quotient; at most 15 (1 + 2^-8) / 16
+        const float t = fmaf(y, 16.f, 96.f);                 // the quotient to 2^-17
+        const uint32_t u = __float_as_uint(t + (kRound - 96.f));
+        code[n] += u << (4 * i);  // 0x4b400000 + c
+      }
+      code[n] -= 0x4b400000u * 0x11111111u;
     }
-    code -= 0x4b400000u * 0x11111111u;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      code |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x.at(i) - m, s)), 0.f), 15.f) << (4 * i);
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        code[n] |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[n].at(i) - m, s)), 0.f), 15.f) << (4 * i);
   }
-  return code;
 }
 
 // The eight values that packed codes and a parameter word stand for, rounded once to T.

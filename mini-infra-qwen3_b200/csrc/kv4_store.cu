@@ -13,6 +13,7 @@ namespace mi {
 namespace {
 
 constexpr int kKv4Threads = 256;
+constexpr int kKv4Tile = 16;  // tokens of a storing CTA
 
 // Eight consecutive elements; 16-byte loads when the host proved them aligned.
 template <typename T, bool VEC>
@@ -29,24 +30,54 @@ __device__ __forceinline__ Raw8<T> kv4_load8(const char* p) {
   return x;
 }
 
-// A CTA takes eight tokens (a quad of lanes each: its slot is looked up once) and strides its warps over
-// the (head, group) pairs, a lane quantising eight values of K and the same eight of V.  A warp's eight
-// tokens of one group read 64-byte runs and, where the tokens share a page, write 128 contiguous bytes.
+// A CTA takes sixteen tokens (two lanes each: its slot is looked up once) and strides its warps over the
+// (head, group) pairs, a lane quantising sixteen values of K and the same of V.  A warp's sixteen tokens of
+// one group read 64-byte runs and, where the tokens share a page, write 256 contiguous bytes.
 // The next pair's loads are issued before this pair is quantised.  NG: groups of a head, 0 for any.
 template <typename T, bool VEC, bool CHUNKS, int NG>
 __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreArgs a) {
   const int lane = threadIdx.x & 31;
   const int warp = threadIdx.x >> 5;
-  const unsigned quad = 0xfu << (lane & 28);
+  const unsigned mates = 0x3u << (lane & 30);
   const unsigned tokens = (unsigned)(CHUNKS ? a.batch * a.padded_len : a.num_tokens);  // < 2^31
-  const unsigned token = blockIdx.x * 8u + (lane >> 2);
-  const bool tell = warp == 0 && blockIdx.y == 0 && (lane & 3) == 0;
-  if (token >= tokens) return;  // the four lanes of a token always take the same path
-  int64_t block, src_k, src_v;
+  const unsigned token = blockIdx.x * (unsigned)kKv4Tile + (lane >> 1);
+  const bool tell = warp == 0 && blockIdx.y == 0 && (lane & 1) == 0;
+  if (token >= tokens) return;  // the two lanes of a token always take the same path
+  const int ng = NG ? NG : a.head_dim / kKv4Group;
+  const int w = lane & 1;  // takes eight-value quarters w and w + 2 of the group
+  const int pairs = a.heads * ng;
+  const int step = gridDim.y * (kKv4Threads / 32);
+  int pair = blockIdx.y * (kKv4Threads / 32) + warp;
+  if (pair >= pairs) return;
+  // where the token comes from; the loads below are in flight while its slot is looked up
+  int64_t row, p;
+  if constexpr (CHUNKS) {
+    row = token / (unsigned)a.padded_len;
+    p = token - (unsigned)row * (unsigned)a.padded_len;
+  } else {
+    row = a.rows ? a.rows[token] : token;
+    p = a.positions ? a.positions[token] : 0;
+    if (row < 0 || row >= a.src_rows || p < 0 || p >= a.src_positions) {
+      if (tell) record_status(MI_STATUS_BAD_INDEX);
+      return;
+    }
+  }
+  const char* k_src = a.k_src + row * a.k_sb[0] + p * a.k_sb[2];
+  const char* v_src = a.v_src + row * a.v_sb[0] + p * a.v_sb[2];
+  auto load = [&](int pair, Raw8<T> (&k)[2], Raw8<T> (&v)[2]) {
+    const int h = pair / ng;
+    const int at = ((pair - h * ng) * kKv4Group + w * 8) * (int)sizeof(T);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      k[n] = kv4_load8<T, VEC>(k_src + h * a.k_sb[1] + at + n * 16 * (int)sizeof(T));
+      v[n] = kv4_load8<T, VEC>(v_src + h * a.v_sb[1] + at + n * 16 * (int)sizeof(T));
+    }
+  };
+  Raw8<T> k[2], v[2];
+  load(pair, k, v);
+  int64_t block;
   unsigned offset;
   if constexpr (CHUNKS) {
-    const unsigned row = token / (unsigned)a.padded_len;
-    const int64_t p = token - row * (unsigned)a.padded_len;
     const int64_t first = a.padded_len - a.chunk_lens[row];
     if (first < 0 && p == 0 && tell) record_status(MI_STATUS_BAD_LENGTH);  // only the last padded_len exist
     if (p < first) return;
@@ -62,63 +93,42 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_store_kernel(const Kv4StoreAr
       if (tell) record_status(MI_STATUS_BAD_BLOCK);
       return;
     }
-    src_k = row * a.k_sb[0] + p * a.k_sb[2];
-    src_v = row * a.v_sb[0] + p * a.v_sb[2];
   } else {
     const int64_t slot = a.slots[token];
     if (slot < 0 || slot >= a.num_blocks * a.block_size) {
       if (tell) record_status(MI_STATUS_BAD_SLOT);
       return;
     }
-    const int64_t row = a.rows ? a.rows[token] : token;
-    const int64_t pos = a.positions ? a.positions[token] : 0;
-    if (row < 0 || row >= a.src_rows || pos < 0 || pos >= a.src_positions) {
-      if (tell) record_status(MI_STATUS_BAD_INDEX);
-      return;
-    }
     block = (unsigned)slot / (unsigned)a.block_size;  // slots < 2^31
     offset = (unsigned)slot - (unsigned)block * (unsigned)a.block_size;
-    src_k = row * a.k_sb[0] + pos * a.k_sb[2];
-    src_v = row * a.v_sb[0] + pos * a.v_sb[2];
   }
-  const int ng = NG ? NG : a.head_dim / kKv4Group;
-  const int w = lane & 3;  // eight-value quarter of the group
   char* k_page = a.k_pool + block * a.heads * a.page_bytes;
   char* v_page = a.v_pool + block * a.heads * a.page_bytes;
   const int par0 = a.block_size * (a.head_dim >> 1) + (int)offset * ng * 4;
-  const int pairs = a.heads * ng;
-  const int step = gridDim.y * (kKv4Threads / 32);
-  auto load = [&](int pair, Raw8<T>& k, Raw8<T>& v) {
-    const int h = pair / ng;
-    const int at = ((pair - h * ng) * kKv4Group + w * 8) * (int)sizeof(T);
-    k = kv4_load8<T, VEC>(a.k_src + src_k + h * a.k_sb[1] + at);
-    v = kv4_load8<T, VEC>(a.v_src + src_v + h * a.v_sb[1] + at);
-  };
-  int pair = blockIdx.y * (kKv4Threads / 32) + warp;
-  if (pair >= pairs) return;
-  Raw8<T> k, v;
-  load(pair, k, v);
   while (true) {
-    Raw8<T> k_next, v_next;
+    Raw8<T> k_next[2], v_next[2];
     const bool more = pair + step < pairs;
     if (more) load(pair + step, k_next, v_next);
-    uint32_t kw, vw;
-    const uint32_t kc = kv4_quantise<T>(k, quad, kw);
-    const uint32_t vc = kv4_quantise<T>(v, quad, vw);
+    uint32_t kw, vw, kc[2], vc[2];
+    kv4_quantise<T>(k, mates, kc, kw);
+    kv4_quantise<T>(v, mates, vc, vw);
     const int h = pair / ng;
     const int g = pair - h * ng;
     const int64_t page = h * a.page_bytes;
     const int64_t code_at = page + ((int64_t)g * a.block_size + offset) * 16 + w * 4;
-    *reinterpret_cast<uint32_t*>(k_page + code_at) = kc;
-    *reinterpret_cast<uint32_t*>(v_page + code_at) = vc;
-    if (w == 0) {
-      *reinterpret_cast<uint32_t*>(k_page + page + par0 + g * 4) = kw;
-      *reinterpret_cast<uint32_t*>(v_page + page + par0 + g * 4) = vw;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      *reinterpret_cast<uint32_t*>(k_page + code_at + n * 8) = kc[n];
+      *reinterpret_cast<uint32_t*>(v_page + code_at + n * 8) = vc[n];
     }
+    *reinterpret_cast<uint32_t*>((w ? v_page : k_page) + page + par0 + g * 4) = w ? vw : kw;
     if (!more) return;
     pair += step;
-    k = k_next;
-    v = v_next;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      k[n] = k_next[n];
+      v[n] = v_next[n];
+    }
   }
 }
 
@@ -189,10 +199,10 @@ __global__ void __launch_bounds__(kKv4Threads) kv4_gather_kernel(const Kv4Gather
 template <typename T>
 cudaError_t launch_kv4_store_t(const Kv4StoreArgs& a, bool chunks, bool vec, cudaStream_t s) {
   const int64_t tokens = chunks ? a.batch * a.padded_len : a.num_tokens;
-  const int64_t tiles = (tokens + 7) / 8;
+  const int64_t tiles = (tokens + kKv4Tile - 1) / kKv4Tile;
   const int pair_tiles = (a.heads * (a.head_dim / kKv4Group) + 7) / 8;
   // every pair of a token in one CTA where the tokens fill the SMs, else the pairs spread over CTAs
-  const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 148 * 8 ? 1 : pair_tiles));
+  const dim3 grid((unsigned)tiles, (unsigned)(tiles >= 148 * 4 ? 1 : pair_tiles));
   auto launch = [&](auto kernel) { kernel<<<grid, kKv4Threads, 0, s>>>(a); };
   const int ng = a.head_dim / kKv4Group;
   if (chunks) {
