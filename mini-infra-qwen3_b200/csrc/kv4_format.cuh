@@ -97,11 +97,10 @@ __device__ __forceinline__ float div15(float x) {
 // word, and the group's parameter word.  `pair` is the mask of the two lanes.
 //
 // An IEEE division per value would bound the store (90 us of a 20,000-token store against 17 us of
-// traffic).  The quotient is (x - m) * (1 / s) instead, off by at most 15.5 * 1.5 * 2^-23 < 2^-18, and
-// ties, which 16-bit values meet every few hundred, are kept exact by rounding it to a multiple of 2^-17
-// first: a quotient within 2^-18 of half way counts as half way (and goes to the even code).  Five
-// instructions a value: difference, product clamped to [0, 1) in units of 16, the two roundings, and the
-// code, the low bits of 1.5 * 2^23 + c, as a digit of the packed word.
+// traffic).  The quotient is the product with 1 / s, corrected once by its residual: it is then off by at
+// most half a unit and 2^-22 of one, so half way points, which 16-bit values meet every few hundred, come
+// out exact.  Six instructions a value: difference, product, residual, correction clamped to [0, 1] in units
+// of 16, rounding, and the code, the low bits of 1.5 * 2^23 + c, as a digit of the packed word.
 template <typename T>
 __device__ __forceinline__ void kv4_quantise(const Raw8<T> (&x)[2], unsigned pair, uint32_t (&code)[2], uint32_t& word) {
   float lo, hi;
@@ -123,14 +122,15 @@ __device__ __forceinline__ void kv4_quantise(const Raw8<T> (&x)[2], unsigned pai
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within 2^-23
     inv *= 0.0625f;
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to an integer
+    const float s16 = 16.f * s;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float y = __saturatef(x[n].less(i, m) * inv);  // a 16th of the quotient; at most 15 (1 + 2^-8) / 16
-        const float t = fmaf(y, 16.f, 96.f);                 // the quotient to 2^-17
-        const uint32_t u = __float_as_uint(t + (kRound - 96.f));
+        const float d = x[n].less(i, m);
+        const float y0 = d * inv;
+        const float y = __saturatef(fmaf(fmaf(-y0, s16, d), inv, y0));  // at most 15 (1 + 2^-8) / 16
+        const uint32_t u = __float_as_uint(fmaf(y, 16.f, 12582912.f));  // 1.5 * 2^23: rounded to an integer
         code[n] += u << (4 * i);  // 0x4b400000 + c
       }
       code[n] -= 0x4b400000u * 0x11111111u;

@@ -139,10 +139,33 @@ def test_chunks_land_in_their_table_slots(starts, lens, width, h, d, bs, dtype):
     assert np.array_equal(kp.cpu().numpy(), want[0]) and np.array_equal(vp.cpu().numpy(), want[1])
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_large_stores_meet_ties_and_near_ties(dtype):
+    """A few million values on a coarse lattice with a sprinkling of tiny ones, which put quotients as near a
+    tie as 16-bit sources can without meeting it: every code is the oracle's."""
+    rng = np.random.default_rng(11)
+    b, h, d, bs = 2000, 8, 128, 16
+    x = rng.standard_normal((b, h, d)) * 1.3
+    x = np.where(rng.random(x.shape) < 0.02, x * 10.0 ** rng.uniform(-6, -3, x.shape), x)
+    k = torch.from_numpy(x).to(DTYPES[dtype]).cuda()
+    kp = torch.zeros((b // bs, h, ops.kv4_page_bytes(bs, d)), dtype=torch.uint8, device="cuda")
+    vp = torch.zeros_like(kp)
+    ops.kv4_scatter(k, k.flip(0), None, None, torch.arange(b).cuda(), kp, vp)
+    want = ko.stored(np64(k))
+    got = ko.read(kp.cpu().numpy(), range(b // bs), bs, d).reshape(b, h, d)
+    other = ko.read(vp.cpu().numpy(), range(b // bs), bs, d).reshape(b, h, d)
+    # x - m and its quotient (at most 15.1) are each rounded by 2^-24 at most: only a quotient nearer a tie than
+    # 15.1 * 2^-23, and not on it, may go the other way
+    _, s, m = ko.quantise(np64(k))
+    exact = (np64(k).reshape(b, h, -1, ko.GROUP) - m[..., None]) / s[..., None].astype(np.float64)
+    away = np.abs(exact - np.floor(exact) - 0.5).reshape(x.shape)
+    assert not ((got != want) & ((away == 0) | (away > 15.1 * 2.0**-23))).any()
+    assert np.array_equal(other[::-1], got)
+
+
 def test_store_of_32_bit_sources_is_at_most_a_near_tie_away():
-    """fp32 sources: a code may differ where the exact quotient is near a tie: x - m is rounded, 2^-24
-    relative, on a quotient up to 15.1; the quotient is computed within 2^-18 and counts as the tie within
-    2^-18 of it: 2^-17 + 2^-20 in all."""
+    """fp32 sources: x - m and its quotient are rounded, so a code may differ where the exact quotient is
+    within 15 * 2^-22 of a tie (two roundings of at most 2^-24 relative, on a quotient up to 15)."""
     rng = np.random.default_rng(1)
     b, h, d, bs = 64, 4, 128, 16
     k = torch.from_numpy(rng.standard_normal((b, h, d)).astype(np.float32)).cuda()
@@ -153,7 +176,7 @@ def test_store_of_32_bit_sources_is_at_most_a_near_tie_away():
     got = ko.read(kp.cpu().numpy(), range(4), bs, d).reshape(b, h, -1, ko.GROUP)
     exact = (np64(k).reshape(got.shape) - m[..., None]) / s[..., None]
     off = np.rint((got - m[..., None]) / s[..., None]) - c
-    tie = np.abs(exact - np.floor(exact) - 0.5) < 2.0**-17 + 2.0**-20
+    tie = np.abs(exact - np.floor(exact) - 0.5) < 15 * 2.0**-22
     assert (off[~tie] == 0).all() and np.abs(off).max() <= 1
     assert torch.equal(kp, vp)
 
