@@ -201,6 +201,8 @@ struct QkNormRopeArgs {
   char* k_pool;
   char* v_pool;
   int64_t num_slots;
+  int64_t page_bytes;  // 4-bit pools: bytes of a page, else 0
+  int block_size;      // 4-bit pools
 };
 cudaError_t launch_qk_norm_rope(const QkNormRopeArgs& a, int dtype, cudaStream_t s);
 

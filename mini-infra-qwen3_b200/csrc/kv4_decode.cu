@@ -17,13 +17,17 @@
 //   * q is scaled by a power of two to a largest value in [2^14, 2^15) and held in fp16: exact for the
 //     16-bit types except far below the row's largest value (absolute error 2^-24 of it).
 //   * p s is held in fp16.  The softmax's running reference is one of p * s, not of p: it keeps the largest
-//     product in fp16's upper range, so rounding costs 2^-12 of a weight; an fp16 model, whose output has
-//     as many bits, carries the rounding's remainder in a second fp16 operand.
+//     product in fp16's upper range, so rounding costs at most 2^-11 of a weight (a group whose step is below
+//     2^-25 of its token's widest loses more of its own); an fp16 model, whose output has as many bits,
+//     carries the rounding's remainder in a second fp16 operand.
 //   * Scores, sums, the minimum terms and O are fp32.
-// grid = (splits, KV head blocks, batch); a producer warp brings whole pages (all heads of the block in
-// one bulk copy for K and one for V) into a ring of shared-memory stages, 4 consumer warps each take a
-// (KV head, 32 tokens) of a stage.  Warps of one KV head merge in shared memory, splits in a second kernel
-// (none where every row is one split).
+// Persistent CTAs, three a SM: a producer warp brings whole pages (all heads of a block in one bulk copy for
+// K and one for V) into a ring of steps of 32 tokens x 4 KV heads (or 64 x 2, 128 x 1), 4 consumer warps each
+// take a (KV head, 32 tokens) of a step.  The sequences' steps form one stream that the CTAs share in equal
+// ranges; pieces of a sequence cut by a border are merged by the combine kernel.
+// Bound by HBM: 64 rows of up to 32,768 tokens, 32/8 heads, 1.36 GB of pages in 223 us, 6.3 TB/s, where a
+// copy reaches 6.55; run for seconds the power limit lowers the clocks and the ALU work of cutting codes shows
+// (266 us).  One CTA per (row, 1,024 tokens) instead took 260 us: its waves ended raggedly.
 //
 // Generic kernel (any type, head_dim, block size and group count): one CTA per (sequence, query head);
 // its warps take the pages in turn, a lane holding value lane of every group, with an online softmax in
@@ -412,378 +416,378 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
   __syncwarp();
 
   while (true) {  // one sequence's share at a time
-  const int n_steps = (int)min(pl.w.rest, (int64_t)(pl.w.steps - pl.w.pos));
-  const int ctx = pl.w.ctx;
-  if (lane == 0 && pl.w.rest > n_steps) pl.next_ctx = pl.w.hb + 1 == nhb ? kv4_ctx(a, pl.w.b + 1) : ctx;
-  int left = min(ctx - pl.w.pos * S::kTokens, n_steps * S::kTokens) - un * kKv4Unit;  // tokens from this unit on
+    const int n_steps = (int)min(pl.w.rest, (int64_t)(pl.w.steps - pl.w.pos));
+    const int ctx = pl.w.ctx;
+    if (lane == 0 && pl.w.rest > n_steps) pl.next_ctx = pl.w.hb + 1 == nhb ? kv4_ctx(a, pl.w.b + 1) : ctx;
+    int left = min(ctx - pl.w.pos * S::kTokens, n_steps * S::kTokens) - un * kKv4Unit;  // tokens from this unit on
 
-  // q as the B operand of S^T: this lane holds column r's values d = 32 g + 8 t + 0..7 of every group.
-  // Column c is query head c % kCols; with SH = 2 the first four columns are for the first tile's
-  // tokens, the last four for the second's.
-  uint32_t qb[NG][4];
-  uint32_t mb[3];  // B operands of the minimum term, see below
-  float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: columns 2t, 2t + 1
-  {
-    float qv[NG][8], qsum[NG];
-    const bool valid = r % kCols < a.groups;
-    const T* qp =
-        reinterpret_cast<const T*>(a.q + pl.w.b * a.q_sb +
-                                   (int64_t)((pl.w.hb * HB + hl) * a.groups + (valid ? r % kCols : 0)) * a.q_sh);
-    float top = 0.f;
+    // q as the B operand of S^T: this lane holds column r's values d = 32 g + 8 t + 0..7 of every group.
+    // Column c is query head c % kCols; with SH = 2 the first four columns are for the first tile's
+    // tokens, the last four for the second's.
+    uint32_t qb[NG][4];
+    uint32_t mb[3];  // B operands of the minimum term, see below
+    float unit[2];   // what one unit of q * (code operand) stands for, times the softmax scale: columns 2t, 2t + 1
+    {
+      float qv[NG][8], qsum[NG];
+      const bool valid = r % kCols < a.groups;
+      const T* qp =
+          reinterpret_cast<const T*>(a.q + pl.w.b * a.q_sb +
+                                     (int64_t)((pl.w.hb * HB + hl) * a.groups + (valid ? r % kCols : 0)) * a.q_sh);
+      float top = 0.f;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      qsum[g] = 0.f;
+      for (int g = 0; g < NG; ++g) {
+        qsum[g] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        qv[g][i] = valid ? Elem<T>::to_f(qp[g * kKv4Group + t * 8 + i]) : 0.f;
-        top = fmaxf(top, fabsf(qv[g][i]));
-        qsum[g] += qv[g][i];
+        for (int i = 0; i < 8; ++i) {
+          qv[g][i] = valid ? Elem<T>::to_f(qp[g * kKv4Group + t * 8 + i]) : 0.f;
+          top = fmaxf(top, fabsf(qv[g][i]));
+          qsum[g] += qv[g][i];
+        }
       }
-    }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e+1)
-    const float up = pow2(14 - e);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = max((int)(__float_as_uint(top) >> 23) - 127, -100);  // 2^e <= top < 2^(e+1)
+      const float up = pow2(14 - e);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
-      qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
-      qsum[g] *= a.scale_log2;
-      float u[8];
+      for (int g = 0; g < NG; ++g) {
+        qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
+        qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
+        qsum[g] *= a.scale_log2;
+        float u[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] = qv[g][i] * up * ((i & 1) ? 0.0625f : 1.f);
-      qb[g][0] = pack2<__half>(u[0], u[4]);
-      qb[g][1] = pack2<__half>(u[1], u[5]);
-      qb[g][2] = pack2<__half>(u[2], u[6]);
-      qb[g][3] = pack2<__half>(u[3], u[7]);
-    }
-    // The minimum term sum_g m_g sum(q_g) as a bf16 MMA on the parameter words themselves: columns 2t
-    // and 2t + 1 of a token's row are (s, m) of group t % NG.  The steps meet zeros; sum(q_g) enters
-    // as three bfloat16s, 24 bits of it: in k 2t + 1, in k 2t + 9 and in a second MMA (NG = 4), or in
-    // k 2t + 1 of both pairs of lanes and in k 2t + 9 (NG = 2).
-    float mine = qsum[0];
+        for (int i = 0; i < 8; ++i) u[i] = qv[g][i] * up * ((i & 1) ? 0.0625f : 1.f);
+        qb[g][0] = pack2<__half>(u[0], u[4]);
+        qb[g][1] = pack2<__half>(u[1], u[5]);
+        qb[g][2] = pack2<__half>(u[2], u[6]);
+        qb[g][3] = pack2<__half>(u[3], u[7]);
+      }
+      // The minimum term sum_g m_g sum(q_g) as a bf16 MMA on the parameter words themselves: columns 2t
+      // and 2t + 1 of a token's row are (s, m) of group t % NG.  The steps meet zeros; sum(q_g) enters
+      // as three bfloat16s, 24 bits of it: in k 2t + 1, in k 2t + 9 and in a second MMA (NG = 4), or in
+      // k 2t + 1 of both pairs of lanes and in k 2t + 9 (NG = 2).
+      float mine = qsum[0];
 #pragma unroll
-    for (int g = 1; g < NG; ++g) mine = (t % NG) == g ? qsum[g] : mine;
-    uint32_t part[3];
+      for (int g = 1; g < NG; ++g) mine = (t % NG) == g ? qsum[g] : mine;
+      uint32_t part[3];
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      part[i] = bf16_bits(mine);
-      mine -= __uint_as_float(part[i] << 16);
+      for (int i = 0; i < 3; ++i) {
+        part[i] = bf16_bits(mine);
+        mine -= __uint_as_float(part[i] << 16);
+      }
+      if constexpr (NG == 4) {
+        mb[0] = part[0] << 16, mb[1] = part[1] << 16, mb[2] = part[2] << 16;
+      } else {
+        mb[0] = (t < 2 ? part[0] : part[1]) << 16, mb[1] = t < 2 ? part[2] << 16 : 0u, mb[2] = 0u;
+      }
+      const float mine_unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
+      unit[0] = __shfl_sync(0xffffffffu, mine_unit, 8 * t);  // accumulator columns 2t, 2t + 1
+      unit[1] = __shfl_sync(0xffffffffu, mine_unit, 8 * t + 4);
     }
-    if constexpr (NG == 4) {
-      mb[0] = part[0] << 16, mb[1] = part[1] << 16, mb[2] = part[2] << 16;
-    } else {
-      mb[0] = (t < 2 ? part[0] : part[1]) << 16, mb[1] = t < 2 ? part[2] << 16 : 0u, mb[2] = 0u;
-    }
-    const float mine_unit = a.scale_log2 * pow2(e) * 1024.f;  // 2^(e - 14) of q, 2^24 of the codes
-    unit[0] = __shfl_sync(0xffffffffu, mine_unit, 8 * t);  // accumulator columns 2t, 2t + 1
-    unit[1] = __shfl_sync(0xffffffffu, mine_unit, 8 * t + 4);
-  }
 
-  float o[D / 16][4];  // O^T: rows are values, columns 2t, 2t + 1
-  float z[NG][2];      // sum p m of this lane's tokens
-  float l[2] = {0.f, 0.f};
-  float ref[2] = {-INFINITY, -INFINITY};
+    float o[D / 16][4];  // O^T: rows are values, columns 2t, 2t + 1
+    float z[NG][2];      // sum p m of this lane's tokens
+    float l[2] = {0.f, 0.f};
+    float ref[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    for (int i = 0; i < D / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 #pragma unroll
-  for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
+    for (int g = 0; g < NG; ++g) z[g][0] = z[g][1] = 0.f;
 
-  for (int it = ctx > 0 ? n_steps : 0; it > 0; --it, left -= S::kTokens) {
-    mbar_wait(&full_bar[st], phase, aborted);
-    if (left > 0) {
-      const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
-      const uint32_t k_mat = smem_u32(k_unit) + mat_row;
-      const uint32_t v_mat = k_mat + HB * S::kPageBytes;
-      const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
+    for (int it = ctx > 0 ? n_steps : 0; it > 0; --it, left -= S::kTokens) {
+      mbar_wait(&full_bar[st], phase, aborted);
+      if (left > 0) {
+        const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
+        const uint32_t k_mat = smem_u32(k_unit) + mat_row;
+        const uint32_t v_mat = k_mat + HB * S::kPageBytes;
+        const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
 #pragma unroll
-      for (int n = 0; n < kSets; ++n) {
-        // ---- scores: x[0..1] token r, x[2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
-        float x[4], wide[2];
-        const uint8_t* k_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4);
-        uint32_t kw[2][NG];
-        kv4_params<NG>(k_par, kw[0]);
-        kv4_params<NG>(k_par + 8 * NG * 4, kw[1]);
-        float y[4], s[4];
+        for (int n = 0; n < kSets; ++n) {
+          // ---- scores: x[0..1] token r, x[2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
+          float x[4], wide[2];
+          const uint8_t* k_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4);
+          uint32_t kw[2][NG];
+          kv4_params<NG>(k_par, kw[0]);
+          kv4_params<NG>(k_par + 8 * NG * 4, kw[1]);
+          float y[4], s[4];
 #pragma unroll
-        for (int i = 0; i < SH; ++i) {  // the minimum term
-          const uint8_t* par = k_unit + (n + i) * (kTilePage + kTileTok * NG * 4) + kPar + (r * NG + t % NG) * 4;
-          const uint32_t w0 = *reinterpret_cast<const uint32_t*>(par);
-          const uint32_t w1 = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4);
-          const uint32_t both[4] = {w0, w1, w0, w1}, once[4] = {w0, w1, 0u, 0u};
-          float u[4];
-          Mma16816<__nv_bfloat16>::zero(u, both, mb[0], mb[1]);
-          if constexpr (NG == 4) Mma16816<__nv_bfloat16>::run(u, once, mb[2], 0u);
+          for (int i = 0; i < SH; ++i) {  // the minimum term
+            const uint8_t* par = k_unit + (n + i) * (kTilePage + kTileTok * NG * 4) + kPar + (r * NG + t % NG) * 4;
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(par);
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(par + 8 * NG * 4);
+            const uint32_t both[4] = {w0, w1, w0, w1}, once[4] = {w0, w1, 0u, 0u};
+            float u[4];
+            Mma16816<__nv_bfloat16>::zero(u, both, mb[0], mb[1]);
+            if constexpr (NG == 4) Mma16816<__nv_bfloat16>::run(u, once, mb[2], 0u);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = i && my_tile == 0 ? y[j] : u[j];
-        }
-#pragma unroll
-        for (int gp = 0; gp < NG / 2; ++gp) {
-          float acc[2][4];
-#pragma unroll
-          for (int i = 0; i < SH; ++i) {
-            uint32_t c[4];
-            ldmatrix_x4(k_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t lo[4], hi[4];
-              kv4_operands(c[2 * j], lo);
-              kv4_operands(c[2 * j + 1], hi);
-              const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
-              const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
-              float u[4];
-              Mma16816<__half>::zero(u, a0, qb[gp * 2 + j][0], qb[gp * 2 + j][1]);
-              Mma16816<__half>::run(u, a1, qb[gp * 2 + j][2], qb[gp * 2 + j][3]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[j][e] = i && my_tile == 0 ? acc[j][e] : u[e];
-            }
+            for (int j = 0; j < 4; ++j) y[j] = i && my_tile == 0 ? y[j] : u[j];
           }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int g = gp * 2 + j;
-            const float s0 = kv4_step(kw[0][g]), s1 = kv4_step(kw[1][g]);
-            s[0] = g ? fmaf(acc[j][0], s0, s[0]) : acc[j][0] * s0;
-            s[1] = g ? fmaf(acc[j][1], s0, s[1]) : acc[j][1] * s0;
-            s[2] = g ? fmaf(acc[j][2], s1, s[2]) : acc[j][2] * s1;
-            s[3] = g ? fmaf(acc[j][3], s1, s[3]) : acc[j][3] * s1;
-          }
-        }
+          for (int gp = 0; gp < NG / 2; ++gp) {
+            float acc[2][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = fmaf(s[j], unit[j & 1], y[j]);
-        // widest step of each token (positive bfloat16s order as integers)
+            for (int i = 0; i < SH; ++i) {
+              uint32_t c[4];
+              ldmatrix_x4(k_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          uint32_t vw[NG];
-          kv4_params<NG>(k_par + HB * S::kPageBytes + j * 8 * NG * 4, vw);
-          uint32_t w = vw[0];
+              for (int j = 0; j < 2; ++j) {
+                uint32_t lo[4], hi[4];
+                kv4_operands(c[2 * j], lo);
+                kv4_operands(c[2 * j + 1], hi);
+                const uint32_t a0[4] = {lo[0], hi[0], lo[1], hi[1]};
+                const uint32_t a1[4] = {lo[2], hi[2], lo[3], hi[3]};
+                float u[4];
+                Mma16816<__half>::zero(u, a0, qb[gp * 2 + j][0], qb[gp * 2 + j][1]);
+                Mma16816<__half>::run(u, a1, qb[gp * 2 + j][2], qb[gp * 2 + j][3]);
 #pragma unroll
-          for (int g = 1; g < NG; ++g) w = __vmaxu2(w, vw[g]);
-          wide[j] = fmaxf(kv4_step(w), kKv4Narrow);
-        }
-        if (tail) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if ((n + my_tile) * 16 + j * 8 + r >= left) {
-              x[2 * j] = x[2 * j + 1] = -INFINITY;
-              wide[j] = kKv4Narrow;
+                for (int e = 0; e < 4; ++e) acc[j][e] = i && my_tile == 0 ? acc[j][e] : u[e];
+              }
             }
-        }
-        // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
-        // then to where the largest p * s of these tokens is 2^11 ----
-        float p[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = ex2_approx(x[j] - ref[j & 1]);
-        const float most = fmaxf(fmaxf(p[0], p[1]) * wide[0], fmaxf(p[2], p[3]) * wide[1]);
-        if (__any_sync(0xffffffffu, most > kKv4Limit)) {
-          const float wl[2] = {log2f(wide[0]) - kKv4TopLog2, log2f(wide[1]) - kKv4TopLog2};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float want = fmaxf(x[c] + wl[0], x[c + 2] + wl[1]);
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
-            want = fmaxf(want, ref[c]);
-            const float base = want == -INFINITY ? 0.f : want;
-            const float alpha = ex2_approx(ref[c] - base);  // 0 from the initial -inf
-            l[c] *= alpha;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              o[i][c] *= alpha;
-              o[i][c + 2] *= alpha;
-            }
-            p[c] = ex2_approx(x[c] - base);
-            p[c + 2] = ex2_approx(x[c + 2] - base);
-            ref[c] = want;
-          }
-        }
-        // ---- O^T += V^T (p s)^T, z += p m ----
-        l[0] += p[0] + p[2];
-        l[1] += p[1] + p[3];
-        const uint8_t* v_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4) + HB * S::kPageBytes;
-        uint32_t vw[2][NG];
-        kv4_params<NG>(v_par, vw[0]);
-        kv4_params<NG>(v_par + 8 * NG * 4, vw[1]);
-        if (tail) {
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            if ((n + my_tile) * 16 + j * 8 + r >= left) {
-#pragma unroll
-              for (int g = 0; g < NG; ++g) vw[j][g] = 0u;
-            }
-        }
-#pragma unroll
-        for (int gp = 0; gp < NG / 2; ++gp) {
-          uint32_t pb[2][kTwo ? 4 : 2];  // p s of the two groups as B operands (and what fp16 left of it)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int g = gp * 2 + j;
-            const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
-            const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
-            z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
-            z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
-            const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
-            const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
-            pb[j][0] = movmatrix_trans(h0);
-            pb[j][1] = movmatrix_trans(h1);
-            if constexpr (kTwo) {
-              const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-              const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-              pb[j][2] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
-              pb[j][3] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < SH; ++i) {
-            uint32_t c[4];
-            ldmatrix_x4_trans(v_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int g = gp * 2 + j;
-              uint32_t lo[4], hi[4];
-              kv4_operands(c[2 * j], lo);
-              kv4_operands(c[2 * j + 1], hi);
-              const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
-              const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
-              uint32_t b[kTwo ? 4 : 2];
+              const float s0 = kv4_step(kw[0][g]), s1 = kv4_step(kw[1][g]);
+              s[0] = g ? fmaf(acc[j][0], s0, s[0]) : acc[j][0] * s0;
+              s[1] = g ? fmaf(acc[j][1], s0, s[1]) : acc[j][1] * s0;
+              s[2] = g ? fmaf(acc[j][2], s1, s[2]) : acc[j][2] * s1;
+              s[3] = g ? fmaf(acc[j][3], s1, s[3]) : acc[j][3] * s1;
+            }
+          }
 #pragma unroll
-              for (int e = 0; e < (kTwo ? 4 : 2); ++e) {
-                const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&pb[j][e]), ones[i]);
-                b[e] = SH == 1 ? pb[j][e] : *reinterpret_cast<const uint32_t*>(&w);
+          for (int j = 0; j < 4; ++j) x[j] = fmaf(s[j], unit[j & 1], y[j]);
+          // widest step of each token (positive bfloat16s order as integers)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t vw[NG];
+            kv4_params<NG>(k_par + HB * S::kPageBytes + j * 8 * NG * 4, vw);
+            uint32_t w = vw[0];
+#pragma unroll
+            for (int g = 1; g < NG; ++g) w = __vmaxu2(w, vw[g]);
+            wide[j] = fmaxf(kv4_step(w), kKv4Narrow);
+          }
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if ((n + my_tile) * 16 + j * 8 + r >= left) {
+                x[2 * j] = x[2 * j + 1] = -INFINITY;
+                wide[j] = kKv4Narrow;
               }
-              Mma16816<__half>::run(o[2 * g], a0, b[0], b[1]);
-              Mma16816<__half>::run(o[2 * g + 1], a1, b[0], b[1]);
+          }
+          // ---- weights p = 2^(x - ref).  A reference moves only when some p * s would leave fp16's range:
+          // then to where the largest p * s of these tokens is 2^11 ----
+          float p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = ex2_approx(x[j] - ref[j & 1]);
+          const float most = fmaxf(fmaxf(p[0], p[1]) * wide[0], fmaxf(p[2], p[3]) * wide[1]);
+          if (__any_sync(0xffffffffu, most > kKv4Limit)) {
+            const float wl[2] = {log2f(wide[0]) - kKv4TopLog2, log2f(wide[1]) - kKv4TopLog2};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float want = fmaxf(x[c] + wl[0], x[c + 2] + wl[1]);
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) want = fmaxf(want, __shfl_xor_sync(0xffffffffu, want, off));
+              want = fmaxf(want, ref[c]);
+              const float base = want == -INFINITY ? 0.f : want;
+              const float alpha = ex2_approx(ref[c] - base);  // 0 from the initial -inf
+              l[c] *= alpha;
+#pragma unroll
+              for (int g = 0; g < NG; ++g) z[g][c] *= alpha;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                o[i][c] *= alpha;
+                o[i][c + 2] *= alpha;
+              }
+              p[c] = ex2_approx(x[c] - base);
+              p[c + 2] = ex2_approx(x[c + 2] - base);
+              ref[c] = want;
+            }
+          }
+          // ---- O^T += V^T (p s)^T, z += p m ----
+          l[0] += p[0] + p[2];
+          l[1] += p[1] + p[3];
+          const uint8_t* v_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4) + HB * S::kPageBytes;
+          uint32_t vw[2][NG];
+          kv4_params<NG>(v_par, vw[0]);
+          kv4_params<NG>(v_par + 8 * NG * 4, vw[1]);
+          if (tail) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if ((n + my_tile) * 16 + j * 8 + r >= left) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g) vw[j][g] = 0u;
+              }
+          }
+#pragma unroll
+          for (int gp = 0; gp < NG / 2; ++gp) {
+            uint32_t pb[2][kTwo ? 4 : 2];  // p s of the two groups as B operands (and what fp16 left of it)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int g = gp * 2 + j;
+              const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
+              const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
+              z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
+              z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
+              const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
+              const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
+              pb[j][0] = movmatrix_trans(h0);
+              pb[j][1] = movmatrix_trans(h1);
               if constexpr (kTwo) {
-                Mma16816<__half>::run(o[2 * g], a0, b[2], b[3]);
-                Mma16816<__half>::run(o[2 * g + 1], a1, b[2], b[3]);
+                const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                pb[j][2] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
+                pb[j][3] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
+              }
+            }
+#pragma unroll
+            for (int i = 0; i < SH; ++i) {
+              uint32_t c[4];
+              ldmatrix_x4_trans(v_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int g = gp * 2 + j;
+                uint32_t lo[4], hi[4];
+                kv4_operands(c[2 * j], lo);
+                kv4_operands(c[2 * j + 1], hi);
+                const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
+                const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
+                uint32_t b[kTwo ? 4 : 2];
+#pragma unroll
+                for (int e = 0; e < (kTwo ? 4 : 2); ++e) {
+                  const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&pb[j][e]), ones[i]);
+                  b[e] = SH == 1 ? pb[j][e] : *reinterpret_cast<const uint32_t*>(&w);
+                }
+                Mma16816<__half>::run(o[2 * g], a0, b[0], b[1]);
+                Mma16816<__half>::run(o[2 * g + 1], a1, b[0], b[1]);
+                if constexpr (kTwo) {
+                  Mma16816<__half>::run(o[2 * g], a0, b[2], b[3]);
+                  Mma16816<__half>::run(o[2 * g + 1], a1, b[2], b[3]);
+                }
               }
             }
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty_bar[st]);
+      if (++st == NST) st = 0, phase ^= 1;
+    }
+
+    if constexpr (SH == 2) {
+      // a head's sums over the first and the second tiles meet: columns 2t and 2t + 4
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float other = __shfl_xor_sync(0xffffffffu, ref[c], 2);
+        const float both = fmaxf(ref[c], other);
+        const float alpha = both == -INFINITY ? 1.f : ex2_approx(ref[c] - both);
+        ref[c] = both;
+        l[c] *= alpha;
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 2);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          z[g][c] *= alpha;
+          z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], 2);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          o[i][c] *= alpha;
+          o[i][c] += __shfl_xor_sync(0xffffffffu, o[i][c], 2);
+          o[i][c + 2] *= alpha;
+          o[i][c + 2] += __shfl_xor_sync(0xffffffffu, o[i][c + 2], 2);
+        }
+      }
+    }
+    // ---- this warp's sums over the lanes that share columns, then its rows: heads 2t, 2t + 1, values
+    // d = 32 g + 4 r + 0..3 (rows r of tile 2g, r + 8 of it, times 16, and of tile 2g + 1) ----
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) {
+        l[c] += __shfl_xor_sync(0xffffffffu, l[c], off);
+#pragma unroll
+        for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
+      }
+    }
+    auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
+    // The rows' outputs where all of the sequence was here, else a partial: slot 0 the CTA's first, 1 its last.
+    const int64_t b = pl.w.b;
+    const int hb = pl.w.hb, pos = pl.w.pos, steps = pl.w.steps;
+    const int taken = (int)min(pl.w.rest, (int64_t)(steps - pos));
+    const int head0 = hb * HB;
+    const int slot = pos == 0 && taken == steps ? -1 : pl.done > 0;
+    if (slot >= 0 && pos == 0 && threadIdx.x == 0) {  // the sequence starts here and is cut: say how often
+      Kv4Cut cut;
+      cut.b = b;
+      cut.hb = hb;
+      cut.slot = slot;
+      const int64_t at = blockIdx.x * pl.quota + pl.done;
+      cut.pieces = (int)((at + steps - 1) / pl.quota - blockIdx.x) + 1;
+      a.cuts[blockIdx.x] = cut;
+    }
+    if (pl.w.ctx == 0) {  // a row of no tokens
+      for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4Consumers * 32)
+        reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
+    } else if constexpr (UN > 1) {
+      // the warps of a KV head merge in shared memory
+      float* so = merge;                             // [warp][column][D]
+      float* sml = so + kKv4Consumers * kCols * D;   // [warp][column](ref, l)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int col = warp * kCols + 2 * t + c;
+        if (2 * t + c >= kCols) continue;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+          *reinterpret_cast<float4*>(so + col * D + g * kKv4Group + r * 4) =
+              make_float4(value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3));
+        if (r == 0) *reinterpret_cast<float2*>(sml + 2 * col) = make_float2(ref[c], l[c]);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");
+      // four values of one (KV head, query head) at a time
+      constexpr int kVec = D / 4;
+      for (int i = threadIdx.x; i < HB * a.groups * kVec; i += kKv4Consumers * 32) {
+        const int row = i / kVec, d = (i - row * kVec) * 4;
+        const int hm = row / a.groups, head = row - hm * a.groups;
+        float m_all = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < UN; ++u) m_all = fmaxf(m_all, sml[2 * ((hm * UN + u) * kCols + head)]);
+        float l_all = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          const int col = (hm * UN + u) * kCols + head;
+          const float f = m_all == -INFINITY ? 1.f : ex2_approx(sml[2 * col] - m_all);
+          l_all = fmaf(f, sml[2 * col + 1], l_all);
+          const float4 x = *reinterpret_cast<const float4*>(so + col * D + d);
+          v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
+        }
+        kv4_emit<T, D>(a, b, (head0 + hm) * a.groups + head, slot, row, d, v, m_all, l_all, d == 0);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");  // before the next sequence's sums
+    } else {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int head = 2 * t + c;
+        if (head >= kCols || head >= a.groups) continue;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const float v[4] = {value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3)};
+          kv4_emit<T, D>(a, b, (head0 + hl) * a.groups + head, slot, hl * a.groups + head, g * kKv4Group + r * 4, v, ref[c], l[c],
+                         g == 0 && r == 0);
+        }
+      }
+    }
+    if (pl.w.rest <= taken) return;
+    __syncwarp();
+    if (lane == 0) {
+      pl.done = pl.done + taken;
+      pl.w.rest = pl.w.rest - taken;
+      pl.w.pos = 0;
+      const bool row_done = hb + 1 == nhb;
+      pl.w.hb = row_done ? 0 : hb + 1;
+      if (row_done) {
+        pl.w.b = b + 1;
+        pl.w.ctx = pl.next_ctx;
+        pl.w.steps = kv4_steps<S::kTokens>(pl.next_ctx);
+      }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&empty_bar[st]);
-    if (++st == NST) st = 0, phase ^= 1;
-  }
-
-  if constexpr (SH == 2) {
-    // a head's sums over the first and the second tiles meet: columns 2t and 2t + 4
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float other = __shfl_xor_sync(0xffffffffu, ref[c], 2);
-      const float both = fmaxf(ref[c], other);
-      const float alpha = both == -INFINITY ? 1.f : ex2_approx(ref[c] - both);
-      ref[c] = both;
-      l[c] *= alpha;
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], 2);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        z[g][c] *= alpha;
-        z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], 2);
-      }
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        o[i][c] *= alpha;
-        o[i][c] += __shfl_xor_sync(0xffffffffu, o[i][c], 2);
-        o[i][c + 2] *= alpha;
-        o[i][c + 2] += __shfl_xor_sync(0xffffffffu, o[i][c + 2], 2);
-      }
-    }
-  }
-  // ---- this warp's sums over the lanes that share columns, then its rows: heads 2t, 2t + 1, values
-  // d = 32 g + 4 r + 0..3 (rows r of tile 2g, r + 8 of it, times 16, and of tile 2g + 1) ----
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-#pragma unroll
-    for (int off = 4; off < 32; off <<= 1) {
-      l[c] += __shfl_xor_sync(0xffffffffu, l[c], off);
-#pragma unroll
-      for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
-    }
-  }
-  auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
-  // The rows' outputs where all of the sequence was here, else a partial: slot 0 the CTA's first, 1 its last.
-  const int64_t b = pl.w.b;
-  const int hb = pl.w.hb, pos = pl.w.pos, steps = pl.w.steps;
-  const int taken = (int)min(pl.w.rest, (int64_t)(steps - pos));
-  const int head0 = hb * HB;
-  const int slot = pos == 0 && taken == steps ? -1 : pl.done > 0;
-  if (slot >= 0 && pos == 0 && threadIdx.x == 0) {  // the sequence starts here and is cut: say how often
-    Kv4Cut cut;
-    cut.b = b;
-    cut.hb = hb;
-    cut.slot = slot;
-    const int64_t at = blockIdx.x * pl.quota + pl.done;
-    cut.pieces = (int)((at + steps - 1) / pl.quota - blockIdx.x) + 1;
-    a.cuts[blockIdx.x] = cut;
-  }
-  if (pl.w.ctx == 0) {  // a row of no tokens
-    for (int i = threadIdx.x; i < HB * a.groups * D; i += kKv4Consumers * 32)
-      reinterpret_cast<T*>(a.out + b * a.out_sb)[(int64_t)head0 * a.groups * D + i] = Elem<T>::from_f(0.f);
-  } else if constexpr (UN > 1) {
-    // the warps of a KV head merge in shared memory
-    float* so = merge;                             // [warp][column][D]
-    float* sml = so + kKv4Consumers * kCols * D;   // [warp][column](ref, l)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int col = warp * kCols + 2 * t + c;
-      if (2 * t + c >= kCols) continue;
-#pragma unroll
-      for (int g = 0; g < NG; ++g)
-        *reinterpret_cast<float4*>(so + col * D + g * kKv4Group + r * 4) =
-            make_float4(value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3));
-      if (r == 0) *reinterpret_cast<float2*>(sml + 2 * col) = make_float2(ref[c], l[c]);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");
-    // four values of one (KV head, query head) at a time
-    constexpr int kVec = D / 4;
-    for (int i = threadIdx.x; i < HB * a.groups * kVec; i += kKv4Consumers * 32) {
-      const int row = i / kVec, d = (i - row * kVec) * 4;
-      const int hm = row / a.groups, head = row - hm * a.groups;
-      float m_all = -INFINITY;
-#pragma unroll
-      for (int u = 0; u < UN; ++u) m_all = fmaxf(m_all, sml[2 * ((hm * UN + u) * kCols + head)]);
-      float l_all = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int col = (hm * UN + u) * kCols + head;
-        const float f = m_all == -INFINITY ? 1.f : ex2_approx(sml[2 * col] - m_all);
-        l_all = fmaf(f, sml[2 * col + 1], l_all);
-        const float4 x = *reinterpret_cast<const float4*>(so + col * D + d);
-        v[0] = fmaf(f, x.x, v[0]), v[1] = fmaf(f, x.y, v[1]), v[2] = fmaf(f, x.z, v[2]), v[3] = fmaf(f, x.w, v[3]);
-      }
-      kv4_emit<T, D>(a, b, (head0 + hm) * a.groups + head, slot, row, d, v, m_all, l_all, d == 0);
-    }
-    asm volatile("bar.sync 1, %0;" ::"n"(kKv4Consumers * 32) : "memory");  // before the next sequence's sums
-  } else {
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int head = 2 * t + c;
-      if (head >= kCols || head >= a.groups) continue;
-#pragma unroll
-      for (int g = 0; g < NG; ++g) {
-        const float v[4] = {value(g, c, 0), value(g, c, 1), value(g, c, 2), value(g, c, 3)};
-        kv4_emit<T, D>(a, b, (head0 + hl) * a.groups + head, slot, hl * a.groups + head, g * kKv4Group + r * 4, v, ref[c], l[c],
-                       g == 0 && r == 0);
-      }
-    }
-  }
-  if (pl.w.rest <= taken) return;
-  __syncwarp();
-  if (lane == 0) {
-    pl.done = pl.done + taken;
-    pl.w.rest = pl.w.rest - taken;
-    pl.w.pos = 0;
-    const bool row_done = hb + 1 == nhb;
-    pl.w.hb = row_done ? 0 : hb + 1;
-    if (row_done) {
-      pl.w.b = b + 1;
-      pl.w.ctx = pl.next_ctx;
-      pl.w.steps = kv4_steps<S::kTokens>(pl.next_ctx);
-    }
-  }
-  __syncwarp();
   }
 }
 

@@ -93,55 +93,101 @@ __device__ __forceinline__ float div15(float x) {
   return fmaf(fmaf(-15.f, q, x), r, q);
 }
 
-// Quantise a group spread over two consecutive lanes (twice eight values each): this lane's codes, eight a
-// word, and the group's parameter word.  `pair` is the mask of the two lanes.
+// A group's parameters from its smallest and largest value, and what its quotients need.
+struct Kv4Scale {
+  float m, s;
+  float inv, s16;  // 1 / (16 s) within 2^-23, 16 s
+  uint32_t word;   // (s, m) as a page holds them
+  bool any;        // false: all codes are 0
+  bool fast;       // s is far from the ends of fp32's range
+};
+__device__ __forceinline__ Kv4Scale kv4_scale(float lo, float hi) {
+  Kv4Scale g;
+  const uint32_t mb = bf16_bits(lo);
+  g.m = __uint_as_float(mb << 16);
+  const uint32_t sb = bf16_bits(div15(hi - g.m));
+  g.s = __uint_as_float(sb << 16);
+  // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
+  const bool spoiled = (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u;
+  // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
+  g.any = !spoiled && g.s > 0.f;
+  g.word = spoiled ? 0x7fc00000u : (mb << 16) | (g.any ? sb : 0u);
+  g.fast = g.s >= 0x1p-110f && g.s <= 0x1p110f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g.inv) : "f"(g.s));
+  g.inv *= 0.0625f;
+  g.s16 = 16.f * g.s;
+  return g;
+}
+
+// round((x - m) / s) clamped to 0..15 as the low bits of 1.5 * 2^23 + c, from d = x - m.
 //
 // An IEEE division per value would bound the store (90 us of a 20,000-token store against 17 us of
 // traffic).  The quotient is the product with 1 / s, corrected once by its residual: it is then off by at
 // most half a unit and 2^-22 of one, so half way points, which 16-bit values meet every few hundred, come
-// out exact.  Six instructions a value: difference, product, residual, correction clamped to [0, 1] in units
-// of 16, rounding, and the code, the low bits of 1.5 * 2^23 + c, as a digit of the packed word.
+// out exact.  Clamped to [0, 1] in units of 16 on the way (at most 15 (1 + 2^-8) / 16 but for the lower end).
+__device__ __forceinline__ uint32_t kv4_code(const Kv4Scale& g, float d) {
+  const float y0 = d * g.inv;
+  const float y = __saturatef(fmaf(fmaf(-y0, g.s16, d), g.inv, y0));
+  return __float_as_uint(fmaf(y, 16.f, 12582912.f));  // rounded to an integer
+}
+constexpr uint32_t kKv4CodeBase = 0x4b400000u;  // 1.5 * 2^23
+
+// The same for steps at the ends of fp32's range: 0..15.
+__device__ __forceinline__ uint32_t kv4_code_slow(const Kv4Scale& g, float d) {
+  return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(d, g.s)), 0.f), 15.f);
+}
+
+// Quantise a group spread over two consecutive lanes (twice eight values each): this lane's codes, eight a
+// word, and the group's parameter word.  `pair` is the mask of the two lanes.
 template <typename T>
 __device__ __forceinline__ void kv4_quantise(const Raw8<T> (&x)[2], unsigned pair, uint32_t (&code)[2], uint32_t& word) {
   float lo, hi;
   kv4_range<T>(x, pair, lo, hi);
+  const Kv4Scale g = kv4_scale(lo, hi);
+  word = g.word;
   code[0] = code[1] = 0u;
-  const uint32_t mb = bf16_bits(lo);
-  const float m = __uint_as_float(mb << 16);
-  const uint32_t sb = bf16_bits(div15(hi - m));
-  const float s = __uint_as_float(sb << 16);
-  // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
-  if ((mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u) {
-    word = 0x7fc00000u;
-    return;
-  }
-  // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
-  word = (mb << 16) | (s > 0.f ? sb : 0u);
-  if (!(s > 0.f)) return;
-  if (s >= 0x1p-110f && s <= 0x1p110f) {
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));  // within 2^-23
-    inv *= 0.0625f;
-    const float s16 = 16.f * s;
+  if (!g.any) return;
+  if (g.fast) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float d = x[n].less(i, m);
-        const float y0 = d * inv;
-        const float y = __saturatef(fmaf(fmaf(-y0, s16, d), inv, y0));  // at most 15 (1 + 2^-8) / 16
-        const uint32_t u = __float_as_uint(fmaf(y, 16.f, 12582912.f));  // 1.5 * 2^23: rounded to an integer
-        code[n] += u << (4 * i);  // 0x4b400000 + c
-      }
-      code[n] -= 0x4b400000u * 0x11111111u;
+      for (int i = 0; i < 8; ++i) code[n] += kv4_code(g, x[n].less(i, g.m)) << (4 * i);
+      code[n] -= kKv4CodeBase * 0x11111111u;  // the digits' common part
     }
   } else {
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        code[n] |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[n].at(i) - m, s)), 0.f), 15.f) << (4 * i);
+      for (int i = 0; i < 8; ++i) code[n] |= kv4_code_slow(g, x[n].at(i) - g.m) << (4 * i);
   }
+}
+
+// Quantise a group spread over 32 / E consecutive lanes, E fp32 values each, by a whole warp: this lane's E
+// codes, packed, and the group's parameter word.  The same bytes as above for the same values.
+template <int E>
+__device__ __forceinline__ uint32_t kv4_quantise_warp(const float (&x)[E], uint32_t& word) {
+  float lo = x[0], hi = x[0], poison = 0.f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    lo = fminf(lo, x[i]);
+    hi = fmaxf(hi, x[i]);
+    poison = fmaf(x[i], 0.f, poison);  // NaN from a NaN (or an infinity)
+  }
+#pragma unroll
+  for (int o = 1; o < 32 / E; o <<= 1) {
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    poison += __shfl_xor_sync(0xffffffffu, poison, o);
+  }
+  const Kv4Scale g = kv4_scale(lo + poison, hi);
+  word = g.word;
+  uint32_t code = 0;
+  if (g.any) {
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      code |= (g.fast ? kv4_code(g, x[i] - g.m) - kKv4CodeBase : kv4_code_slow(g, x[i] - g.m)) << (4 * i);
+  }
+  return code;
 }
 
 // The eight values that packed codes and a parameter word stand for, rounded once to T.

@@ -18,6 +18,7 @@
 // the fp32 statistic by at most a few ulp.
 #include "common.cuh"
 #include "kernels.cuh"
+#include "kv4_format.cuh"
 
 namespace mi {
 namespace {
@@ -107,7 +108,8 @@ __global__ void __launch_bounds__(kNormThreads) rmsnorm_kernel(const RmsNormArgs
 
 // One warp per (token, head); lane l owns elements [l*EPL, l*EPL + EPL) of head_dim = 32*EPL, so
 // the rotate-half partner of lane l is lane l ^ 16.
-template <typename T, int EPL>
+// With KV4 the append goes to 4-bit pages: a group of 32 values lies in 32 / EPL neighbouring lanes.
+template <typename T, int EPL, bool KV4>
 __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const QkNormRopeArgs a) {
   const int64_t wid = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
@@ -154,9 +156,35 @@ __global__ void __launch_bounds__(128) qk_norm_rope_kernel(const QkNormRopeArgs 
       if (lane == 0) record_status(MI_STATUS_BAD_SLOT);
       return;
     }
-    const int64_t off = (slot * a.hkv + kh) * D + e0;
-    store_vec<T, EPL>(reinterpret_cast<T*>(a.k_pool) + off, o);
-    store_vec<T, EPL>(reinterpret_cast<T*>(a.v_pool) + off, v);
+    if constexpr (KV4) {
+      const int64_t block = slot / a.block_size;
+      const int offset = (int)(slot - block * a.block_size);
+      const int64_t page = (block * a.hkv + kh) * a.page_bytes;
+      const int64_t at = page + ((int64_t)(e0 / kKv4Group) * a.block_size + offset) * 16 + e0 % kKv4Group / 2;
+      const int64_t par_at = page + (int64_t)a.block_size * (D / 2) + (offset * (D / kKv4Group) + e0 / kKv4Group) * 4;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        float x[EPL];
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) x[i] = kv ? v[i] : round_t<T>(o[i]);
+        uint32_t word;
+        uint32_t code = kv4_quantise_warp<EPL>(x, word);
+        char* pool = kv ? a.v_pool : a.k_pool;
+        if constexpr (EPL == 8) {
+          *reinterpret_cast<uint32_t*>(pool + at) = code;
+        } else if constexpr (EPL == 4) {
+          *reinterpret_cast<uint16_t*>(pool + at) = (uint16_t)code;
+        } else {
+          if constexpr (EPL == 1) code |= __shfl_down_sync(0xffffffffu, code, 1) << 4;
+          if (EPL == 2 || (lane & 1) == 0) *reinterpret_cast<uint8_t*>(pool + at) = (uint8_t)code;
+        }
+        if (e0 % kKv4Group == 0) *reinterpret_cast<uint32_t*>(pool + par_at) = word;
+      }
+    } else {
+      const int64_t off = (slot * a.hkv + kh) * D + e0;
+      store_vec<T, EPL>(reinterpret_cast<T*>(a.k_pool) + off, o);
+      store_vec<T, EPL>(reinterpret_cast<T*>(a.v_pool) + off, v);
+    }
   }
 }
 
@@ -196,15 +224,15 @@ cudaError_t launch_rmsnorm_t(const RmsNormArgs& a, bool vec16, cudaStream_t s) {
   return launch_rmsnorm_v<T, 1>(a, s);
 }
 
-template <typename T>
+template <typename T, bool KV4>
 cudaError_t launch_qk_norm_rope_t(const QkNormRopeArgs& a, cudaStream_t s) {
   const int64_t warps = a.tokens * (a.hq + a.hkv);
   const dim3 grid((unsigned)((warps + 3) / 4));
   switch (a.head_dim) {
-    case 32: qk_norm_rope_kernel<T, 1><<<grid, 128, 0, s>>>(a); break;
-    case 64: qk_norm_rope_kernel<T, 2><<<grid, 128, 0, s>>>(a); break;
-    case 128: qk_norm_rope_kernel<T, 4><<<grid, 128, 0, s>>>(a); break;
-    case 256: qk_norm_rope_kernel<T, 8><<<grid, 128, 0, s>>>(a); break;
+    case 32: qk_norm_rope_kernel<T, 1, KV4><<<grid, 128, 0, s>>>(a); break;
+    case 64: qk_norm_rope_kernel<T, 2, KV4><<<grid, 128, 0, s>>>(a); break;
+    case 128: qk_norm_rope_kernel<T, 4, KV4><<<grid, 128, 0, s>>>(a); break;
+    case 256: qk_norm_rope_kernel<T, 8, KV4><<<grid, 128, 0, s>>>(a); break;
     default: return cudaErrorInvalidValue;
   }
   return cudaGetLastError();
@@ -232,9 +260,14 @@ cudaError_t launch_rmsnorm(const RmsNormArgs& a, bool vec16, int dtype, cudaStre
 
 cudaError_t launch_qk_norm_rope(const QkNormRopeArgs& a, int dtype, cudaStream_t s) {
   if (a.tokens == 0) return cudaSuccess;
-  if (dtype == MI_BF16) return launch_qk_norm_rope_t<__nv_bfloat16>(a, s);
-  if (dtype == MI_F16) return launch_qk_norm_rope_t<__half>(a, s);
-  return launch_qk_norm_rope_t<float>(a, s);
+  if (a.slots && a.page_bytes) {
+    if (dtype == MI_BF16) return launch_qk_norm_rope_t<__nv_bfloat16, true>(a, s);
+    if (dtype == MI_F16) return launch_qk_norm_rope_t<__half, true>(a, s);
+    return launch_qk_norm_rope_t<float, true>(a, s);
+  }
+  if (dtype == MI_BF16) return launch_qk_norm_rope_t<__nv_bfloat16, false>(a, s);
+  if (dtype == MI_F16) return launch_qk_norm_rope_t<__half, false>(a, s);
+  return launch_qk_norm_rope_t<float, false>(a, s);
 }
 
 cudaError_t launch_silu_mul(const SiluMulArgs& a, bool vec16, int dtype, cudaStream_t s) {

@@ -1,6 +1,7 @@
 // Whole blocks copied inside every pool of the cache: (src, dst) pairs x pools in one launch.
 //
-// Pure data movement, 2 * block_bytes of HBM traffic per pair and pool.  One CTA per (pair, pool).
+// Pure data movement, 2 * block_bytes of HBM traffic per pair and pool.  One CTA per (pair, pool): 512 blocks of
+// 32 KiB in 56 pools take 284 us, 6.6 TB/s, the rate of a plain copy; 3 blocks 5.4 us.
 #include "common.cuh"
 #include "kernels.cuh"
 
