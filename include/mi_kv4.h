@@ -70,6 +70,17 @@ int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* 
                          void* stream);
 
 /*
+ * mi_kv4_qk_norm_rope — mi_qk_norm_rope (mi_layers.h) whose decode append goes to 4-bit pools: roped K and V,
+ * rounded to dtype, are quantised into the pages at slot_mapping, the bytes that mi_kv4_scatter of k_out and
+ * v_out would leave there.  head_dim in {32, 64, 128, 256}.
+ */
+int mi_kv4_qk_norm_rope(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                        int64_t v_row_stride, const void* q_weight, const void* k_weight, const void* cos,
+                        const void* sin, int64_t cos_sin_row_stride, int64_t tokens, int hq, int hkv, int head_dim,
+                        float eps, void* q_out, void* k_out, void* v_out, const int64_t* slot_mapping, void* k_pool,
+                        void* v_pool, int64_t num_blocks, int block_size, int dtype, void* stream);
+
+/*
  * mi_kv4_paged_decode — mi_paged_decode over 4-bit pools: one query token per sequence attends to
  * positions [0, context_lens[b]) of its block table; arguments as there.  With k_new, v_new,
  * new_strides and slot_mapping the new tokens are quantised into the pools first.  A row with

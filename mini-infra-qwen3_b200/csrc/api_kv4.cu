@@ -155,6 +155,19 @@ int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* 
   return e == cudaSuccess ? MI_OK : cuda_fail(e, "mi_kv4_gather_blocks launch");
 }
 
+int mi_kv4_qk_norm_rope(const void* q, int64_t q_row_stride, const void* k, int64_t k_row_stride, const void* v,
+                        int64_t v_row_stride, const void* q_weight, const void* k_weight, const void* cos,
+                        const void* sin, int64_t cos_sin_row_stride, int64_t tokens, int hq, int hkv, int head_dim,
+                        float eps, void* q_out, void* k_out, void* v_out, const int64_t* slot_mapping, void* k_pool,
+                        void* v_pool, int64_t num_blocks, int block_size, int dtype, void* stream) {
+  if (int rc = check_kv4_geometry(num_blocks, block_size, hkv, head_dim, dtype, k_pool, v_pool)) return rc;
+  if (tokens > 0 && !slot_mapping) return fail(MI_ERR_INVALID, "mi_kv4_qk_norm_rope: null slot_mapping");
+  return qk_norm_rope_impl(q, q_row_stride, k, k_row_stride, v, v_row_stride, q_weight, k_weight, cos, sin,
+                           cos_sin_row_stride, tokens, hq, hkv, head_dim, eps, q_out, k_out, v_out, slot_mapping, k_pool,
+                           v_pool, num_blocks * block_size, mi_kv4_page_bytes(block_size, head_dim), block_size, dtype,
+                           stream);
+}
+
 size_t mi_kv4_paged_decode_workspace_size(int64_t batch, int num_q_heads, int num_kv_heads, int head_dim,
                                           int64_t max_blocks_per_seq, int block_size, int dtype) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_blocks_per_seq <= 0 ||

@@ -61,6 +61,11 @@ SIGNATURES: dict[str, tuple] = {
     "mi_kv4_scatter": (_I, [_P, _P, _I64P, _I64P, _L, _L, _P, _P, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
     "mi_kv4_store_chunks": (_I, [_P, _P, _I64P, _I64P, _L, _L, _P, _P, _P, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
     "mi_kv4_gather_blocks": (_I, [_P, _P, _P, _L, _P, _I, _L, _L, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "mi_kv4_qk_norm_rope": (
+        _I,
+        [_P, _L, _P, _L, _P, _L, _P, _P, _P, _P, _L, _L, _I, _I, _I, ctypes.c_float, _P, _P, _P, _P, _P, _P, _L, _I, _I,
+         _P],
+    ),
     "mi_kv4_paged_decode_workspace_size": (ctypes.c_size_t, [_L, _I, _I, _I, _L, _I, _I]),
     "mi_kv4_paged_decode": (
         _I,

@@ -25,7 +25,7 @@ Tensor layout inside the model: activations [B, L, hidden]; Q/K/V [B, L, heads, 
 Present K/V returned by prefill are [B, H_kv, L, D] views (the reference's ``KVCache`` layout).
 
 With 4-bit pools (uint8 pages, ``PagedKV4CachePool``) the same two forms run on ``mi_kv4_paged_decode``,
-after the store that quantises the new K/V, and on the dense gather of the history's blocks followed by
+after ``mi_kv4_qk_norm_rope`` has quantised the new K/V, and on the dense gather of the history's blocks followed by
 ``mi_paged_prefill``.
 
 Head partition (``tp_world > 1``): the layer keeps query heads [r*Hq/P, (r+1)*Hq/P) and KV heads
@@ -238,11 +238,10 @@ class Qwen3Attention(nn.Module):
         return self.o_proj(attn), present
 
     def _decode_kv4(self, q, k, v, cos2, sin2, kv_pool: PastKeyValue, md: PagedAttentionMetadata, out=None):
-        """Decode rows over 4-bit pools: norm + RoPE, then the new K/V quantised into the pools and attended to."""
-        q_out, k_out, v_out = ops.qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos2, sin2,
-                                               self.q_norm.eps, self.num_heads, self.num_kv_heads)
-        return ops.kv4_paged_decode(q_out, *kv_pool, md.block_tables, md.context_lens, self.scaling, key_new=k_out,
-                                    value_new=v_out, slot_mapping=md.slot_mapping, out=out)
+        """Decode rows over 4-bit pools: norm + RoPE and the new K/V quantised into the pools in one launch."""
+        q_out = ops.kv4_qk_norm_rope(q, k, v, self.q_norm.weight, self.k_norm.weight, cos2, sin2, self.q_norm.eps,
+                                     self.num_heads, self.num_kv_heads, md.slot_mapping, *kv_pool)
+        return ops.kv4_paged_decode(q_out, *kv_pool, md.block_tables, md.context_lens, self.scaling, out=out)
 
     def _mixed(self, q, k, v, cos2, sin2, kv_pool, md: "MixedMetadata", b: int, length: int):
         """Decode rows [0, nd) through the fused append + paged decode, chunk rows through the

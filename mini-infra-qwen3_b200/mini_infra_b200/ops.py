@@ -767,3 +767,42 @@ def kv4_paged_prefill(
     dense = torch.arange(b * nb, device=query.device).view(b, nb)
     return paged_prefill(query, key_chunk, value_chunk, key.flatten(0, 1), value.flatten(0, 1), dense, start_positions,
                          chunk_lens, scale, out=out)
+
+
+def kv4_qk_norm_rope(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    eps: float,
+    num_q_heads: int,
+    num_kv_heads: int,
+    slot_mapping: torch.Tensor,
+    k_pool: torch.Tensor,
+    v_pool: torch.Tensor,
+) -> torch.Tensor:
+    """``qk_norm_rope`` with its decode append into 4-bit pools (head_dim 32, 64, 128 or 256): returns q_out
+    [T, Hq, D]; the roped K and the V of token t are quantised into slot slot_mapping[t]."""
+    device = _require_cuda("kv4_qk_norm_rope", q, k, v, q_weight, k_weight, cos, sin, slot_mapping, k_pool, v_pool)
+    q2, k2, v2, c2, s2 = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _rows(cos, "cos"), _rows(sin, "sin")
+    if c2.stride(0) != s2.stride(0):
+        c2, s2 = c2.contiguous(), s2.contiguous()
+    tokens, d = q2.shape[0], int(q_weight.shape[0])
+    n, bs, h = _check_kv4(k_pool, v_pool, d)
+    slots = _index(slot_mapping, "slot_mapping")
+    if (h != num_kv_heads or slots.numel() != tokens or k2.shape != (tokens, h * d) or v2.shape != k2.shape
+            or q2.shape[1] != num_q_heads * d or c2.shape != (tokens, d) or s2.shape != c2.shape):
+        raise ValueError(f"{tokens} tokens of {num_q_heads} query and {num_kv_heads} KV heads x {d}, cos and sin of {d} and "
+                         f"one slot each do not fit q {tuple(q2.shape)}, k {tuple(k2.shape)}, v {tuple(v2.shape)}, "
+                         f"cos {tuple(c2.shape)}, sin {tuple(s2.shape)}, {slots.numel()} slots and pools of {h} heads")
+    if any(t.dtype != q.dtype for t in (k, v, q_weight, k_weight, cos, sin)):
+        raise ValueError(f"every dense operand must be {q.dtype}")
+    q_out = torch.empty((tokens, num_q_heads, d), dtype=q.dtype, device=device)
+    _launch(device, "mi_kv4_qk_norm_rope", q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(),
+            v2.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), c2.data_ptr(), s2.data_ptr(), c2.stride(0), tokens,
+            num_q_heads, num_kv_heads, d, float(eps), q_out.data_ptr(), None, None, slots.data_ptr(), k_pool.data_ptr(),
+            v_pool.data_ptr(), n, bs, dtype_code(q.dtype))
+    return q_out

@@ -236,6 +236,36 @@ def test_bad_slots_rows_lengths_and_blocks_are_flagged_and_skipped():
     assert key[0, 0].any() and not key[0, 1].any() and not key[1].any() and not value[1].any()
 
 
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_append_fused_with_norm_and_rope_leaves_the_scatters_bytes(d, dtype):
+    """Against mi_qk_norm_rope's own outputs scattered, q included; packed projections, a bad slot, a NaN."""
+    rng = np.random.default_rng(d)
+    t, hq, h, bs, n = 7, 4, 2, 16, 3
+    qkv = tokens(rng, (t, (hq + 2 * h) * d), dtype)
+    q, k, v = qkv[:, : hq * d], qkv[:, hq * d : (hq + h) * d], qkv[:, (hq + h) * d :]
+    v[3, 5] = float("nan")
+    v[4] = 0.5
+    qw, kw = tokens(rng, (d,), dtype), tokens(rng, (d,), dtype)
+    cos, sin = tokens(rng, (t, d), dtype), tokens(rng, (t, d), dtype)
+    slots = torch.tensor([5, 17, 0, 47, 30, 31, n * bs]).cuda()
+    fused = [torch.zeros((n, h, ops.kv4_page_bytes(bs, d)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    apart = [p.clone() for p in fused]
+    got = ops.kv4_qk_norm_rope(q, k, v, qw, kw, cos, sin, 1e-6, hq, h, slots, *fused)
+    assert ops.read_status() == nat.MI_STATUS_BAD_SLOT
+    want, k_out, v_out = ops.qk_norm_rope(q, k, v, qw, kw, cos, sin, 1e-6, hq, h)
+    ops.kv4_scatter(k_out[:6], v_out[:6], None, None, slots[:6], *apart)
+    assert ops.read_status() == 0
+    assert torch.equal(got, want) and torch.equal(fused[0], apart[0]) and torch.equal(fused[1], apart[1])
+    for args in [(q, k, v, qw, kw, cos, sin, 1e-6, hq, h, slots[:6], *fused),
+                 (q, k[:, :d], v, qw, kw, cos, sin, 1e-6, hq, h, slots, *fused),
+                 (q, k, v, qw, kw, cos[:3], sin[:3], 1e-6, hq, h, slots, *fused),
+                 (q, k, v, qw, kw, cos.double(), sin, 1e-6, hq, h, slots, *fused),
+                 (q, k, v, qw, kw, cos, sin, 1e-6, hq, h, slots, fused[0][:, :1], fused[1][:, :1])]:
+        with pytest.raises(ValueError):
+            ops.kv4_qk_norm_rope(*args)
+
+
 # ---------------------------------------------------------------------------------------------
 # gather
 # ---------------------------------------------------------------------------------------------

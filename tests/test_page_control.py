@@ -204,6 +204,15 @@ def test_host_rejects_bad_arguments_before_launch():
     assert decode(batch=70000) == nat.MI_ERR_UNSUPPORTED and decode(batch=0) == nat.MI_OK
     assert decode(width=4096, stride=4096) == nat.MI_ERR_INVALID and "workspace" in nat.last_error()
 
+    def append(slots=fine, d=128, bs=16, pool=fine):
+        return lib.mi_kv4_qk_norm_rope(fine, 0, fine, 0, fine, 0, fine, fine, fine, fine, 0, 2, 16, 8, d, ctypes.c_float(1e-6),
+                                       None, None, None, slots, pool, pool, 8, bs, nat.MI_BF16, None)
+
+    assert append(slots=None) == nat.MI_ERR_INVALID and "slot_mapping" in nat.last_error()
+    assert append(d=96) == nat.MI_ERR_UNSUPPORTED and append(bs=0) == nat.MI_ERR_INVALID
+    assert append() == nat.MI_ERR_INVALID and "null pointer" in nat.last_error()  # q_out
+    assert append(pool=None) == nat.MI_ERR_INVALID
+
     pools = (ctypes.c_void_p * 2)(256, None)
     assert lib.mi_kv_copy_blocks(pools, 2, fine, 3, 8, 64, None) == nat.MI_ERR_INVALID
     assert lib.mi_kv_copy_blocks(None, 2, fine, 3, 8, 64, None) == nat.MI_ERR_INVALID
