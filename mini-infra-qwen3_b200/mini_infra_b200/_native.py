@@ -9,10 +9,12 @@ reference's shape checks), the other codes become ``RuntimeError``.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
-from mini_infra_b200.build import LIB_PATH
+from mini_infra_b200.build import CALLS_PATH, LIB_PATH
 
 MI_F32, MI_BF16, MI_F16 = 0, 1, 2
 MI_OK, MI_ERR_INVALID, MI_ERR_CUDA, MI_ERR_UNSUPPORTED = 0, -1, -2, -3
@@ -109,6 +111,27 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = argtypes
             _lib = lib
     return _lib
+
+
+_calls = None
+
+
+def calls():
+    """The CPython extension over the library (``csrc/torch_calls.cpp``), loaded once."""
+    global _calls
+    if _calls is None:
+        load()
+        with _lock:
+            if not CALLS_PATH.exists():
+                raise RuntimeError(f"{CALLS_PATH.name} not found at {CALLS_PATH}; build it with "
+                                   "`python -m mini_infra_b200.build`")
+            import torch  # noqa: F401  (its libraries resolve the extension's symbols)
+
+            loader = importlib.machinery.ExtensionFileLoader("_mi_calls", str(CALLS_PATH))
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mi_calls", loader))
+            loader.exec_module(module)
+            _calls = module
+    return _calls
 
 
 def last_error() -> str:

@@ -8,10 +8,7 @@ per-device buffer that grows on demand (the library itself never allocates).
 
 from __future__ import annotations
 
-import array
 import ctypes
-import itertools
-import operator
 from collections.abc import Sequence
 
 import torch
@@ -503,13 +500,14 @@ def decode_rows(
 # ---------------------------------------------------------------------------------------------
 # Block copies and the 4-bit paged cache (include/mi_kv4.h).  These run on the current stream of
 # the tensors' device, which need not be the current device; their workspaces come from PyTorch's
-# allocator at each call, so calls on different streams and captured graphs share none.
+# allocator at each call, so calls on different streams and captured graphs share none.  The ordinary call
+# goes through the CPython extension (``nat.calls()``, ``csrc/torch_calls.cpp``), which answers None for
+# anything else; what follows then handles it or says what is wrong with it.
 # ---------------------------------------------------------------------------------------------
 KV4_GROUP = 32  # values along head_dim that share a step and a minimum
 
 
 _A2, _A3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
-_NBYTES = operator.attrgetter("nbytes")
 
 
 def _launch(device: torch.device, name: str, *args) -> None:
@@ -533,26 +531,26 @@ def kv_copy_blocks(pools: Sequence[torch.Tensor], pairs: torch.Tensor) -> None:
     type, 4-bit pages among them.  Destinations must be distinct and not be sources of other pairs
     (nothing orders the pairs; ``PagedKVCachePool.copy_blocks`` checks that); (b, b) does nothing.
     Ids out of range are skipped and set MI_STATUS_BAD_BLOCK."""
+    if nat.calls().kv_copy_blocks(pools, pairs):
+        return
     device = _require_cuda("kv_copy_blocks", pairs)
     if pairs.dtype != torch.int64 or pairs.ndim != 2 or pairs.shape[1] != 2:
         raise ValueError(f"pairs must be int64 [n, 2], got {tuple(pairs.shape)} {pairs.dtype}")
     if not pools:
         return
-    # a pool per layer, K and V: C-level maps, a Python loop over them would cost more than the copy
     first = pools[0]
     size = first.nbytes
-    if set(map(torch.Tensor.get_device, pools)) != {device.index}:
-        _require_cuda("kv_copy_blocks", pairs, *pools)
-    if (first.ndim < 2 or set(map(_NBYTES, pools)) != {size} or not all(map(torch.Tensor.is_contiguous, pools))
-            or set(map(torch.Tensor.size, pools, itertools.repeat(0))) != {first.shape[0]}):
+    _require_cuda("kv_copy_blocks", pairs, *pools)
+    if first.ndim < 2 or any(p.ndim < 2 or p.shape[0] != first.shape[0] or p.nbytes != size or not p.is_contiguous()
+                             for p in pools):
         raise ValueError("pools must be contiguous [num_blocks, ...] tensors of the same blocks and bytes")
     blocks = first.shape[0]
     if blocks == 0 or size == 0:
         return
     if not pairs.is_contiguous():
         pairs = pairs.contiguous()
-    table = array.array("Q", map(torch.Tensor.data_ptr, pools))
-    _launch(device, "mi_kv_copy_blocks", table.buffer_info()[0], len(pools), pairs.data_ptr(), pairs.shape[0], blocks, size // blocks)
+    table = (ctypes.c_void_p * len(pools))(*[p.data_ptr() for p in pools])
+    _launch(device, "mi_kv_copy_blocks", table, len(pools), pairs.data_ptr(), pairs.shape[0], blocks, size // blocks)
 
 
 def kv4_page_bytes(block_size: int, head_dim: int) -> int:
@@ -588,6 +586,8 @@ def kv4_scatter(
 ) -> None:
     """``kv_scatter`` into 4-bit pools: token i = src[token_rows[i], :, token_positions[i], :] of K and V is
     quantised into slot slot_mapping[i].  key/value: [B, H, L, D], or [B, H, D] with both index tensors None."""
+    if token_rows is None and token_positions is None and nat.calls().kv4_append(key, value, slot_mapping, k_pool, v_pool):
+        return
     device = _require_cuda("kv4_scatter", key, value, slot_mapping, k_pool, v_pool, token_rows, token_positions)
     if key.shape != value.shape or key.ndim not in (3, 4) or key.dtype != value.dtype:
         raise ValueError(f"key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} must be "
@@ -628,6 +628,8 @@ def kv4_store_chunks(
 ) -> None:
     """``kv_store_chunks`` into 4-bit pools: each row's right-aligned chunk tokens (key/value [B, H, L, D]) are
     quantised at their table slots."""
+    if nat.calls().kv4_store_chunks(key, value, chunk_lens, start_positions, block_tables, k_pool, v_pool):
+        return
     device = _require_cuda("kv4_store_chunks", key, value, chunk_lens, start_positions, block_tables, k_pool, v_pool)
     if key.shape != value.shape or key.ndim != 4 or key.dtype != value.dtype:
         raise ValueError(f"key {tuple(key.shape)} {key.dtype} and value {tuple(value.shape)} {value.dtype} must be "
@@ -658,6 +660,10 @@ def kv4_gather_blocks(
     """Blocks of 4-bit pools as dense ones: (key, value), each [B, nb, bs, H, D] in `dtype` for block_ids
     [B, nb].  With lengths [B], row b's tokens at and past lengths[b] are zeros and the ids of blocks past
     it are not read; fill_past=False leaves those blocks uninitialised."""
+    code = dtype_code(dtype)
+    got = nat.calls().kv4_gather_blocks(k_pool, v_pool, block_ids, head_dim, code, lengths, fill_past)
+    if got is not None:
+        return got
     device = _require_cuda("kv4_gather_blocks", k_pool, v_pool, block_ids, lengths)
     n, bs, h = _check_kv4(k_pool, v_pool, head_dim)
     if block_ids.dtype != torch.int64 or block_ids.ndim != 2:
@@ -668,7 +674,6 @@ def kv4_gather_blocks(
         lengths = _index(lengths, "lengths")
         if lengths.numel() != b:
             raise ValueError(f"lengths has {lengths.numel()} entries for {b} rows")
-    code = dtype_code(dtype)
     key = torch.empty((b, nb, bs, h, head_dim), dtype=dtype, device=device)
     value = torch.empty_like(key)
     _launch(device, "mi_kv4_gather_blocks", k_pool.data_ptr(), v_pool.data_ptr(), ids.data_ptr(),
@@ -694,6 +699,10 @@ def kv4_paged_decode(
 
     With key_new/value_new/slot_mapping the new token's K/V ([B, H, D]) are quantised into the pools
     first, so that the row attends to them as the cache holds them."""
+    if key_new is None and value_new is None and slot_mapping is None and out is None and ws is None:
+        got = nat.calls().kv4_paged_decode(query, k_pool, v_pool, block_tables, context_lens, scale)
+        if got is not None:
+            return got
     device = _require_cuda("kv4_paged_decode", query, k_pool, v_pool, block_tables, context_lens, key_new, value_new,
                            slot_mapping, out, ws)
     if query.ndim != 3:

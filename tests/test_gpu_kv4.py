@@ -614,6 +614,47 @@ def test_two_streams_and_a_captured_graph_share_no_workspace():
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(again, want[0])
 
 
+def test_the_ordinary_call_and_the_general_one_agree():
+    """Plain contiguous operands go through the CPython extension, others (here: an output of one's own, a
+    strided id or length tensor, index tensors) through ctypes: the same results, bit for bit."""
+    q, kp, vp, tables, ctx = decode_case(6, 16, 8, 128, 16, (1, 900), "bf16")
+    kp, vp, tables, ctx = cuda(kp), cuda(vp), cuda(tables), cuda(ctx)
+    calls = nat.calls()
+    quick = calls.kv4_paged_decode(q, kp, vp, tables, ctx, 0.1)
+    assert quick is not None
+    assert torch.equal(quick, ops.kv4_paged_decode(q, kp, vp, tables, ctx, 0.1, out=torch.empty_like(quick)))
+    ids = tables[:, :3].contiguous()
+    wide = torch.zeros((6, 6), dtype=torch.long, device="cuda")
+    wide[:, ::2] = ids
+    quick = calls.kv4_gather_blocks(kp, vp, ids, 128, nat.MI_F16, ctx, True)
+    assert calls.kv4_gather_blocks(kp, vp, wide[:, ::2], 128, nat.MI_F16, ctx, True) is None
+    general = ops.kv4_gather_blocks(kp, vp, wide[:, ::2], 128, torch.float16, lengths=ctx)
+    assert torch.equal(quick[0], general[0]) and torch.equal(quick[1], general[1])
+    k = q[:, :8]
+    slots, rows = torch.arange(6).cuda(), torch.arange(6).cuda()
+    a, b = [kp.clone(), vp.clone()], [kp.clone(), vp.clone()]
+    assert calls.kv4_append(k, k, slots, *a)
+    ops.kv4_scatter(k[:, :, None], k[:, :, None], rows, None, slots, *b)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = k[:, :, None]
+    one = torch.ones(6, dtype=torch.long, device="cuda")
+    spread = torch.ones(12, dtype=torch.long, device="cuda")[::2]
+    own = torch.arange(1, 7).cuda()[:, None]
+    assert calls.kv4_store_chunks(x, x, one, one, own, *a)
+    assert calls.kv4_store_chunks(x, x, spread, one, own, *b) is None
+    ops.kv4_store_chunks(x, x, spread, one, own, *b)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    pairs = torch.tensor([[1, 8], [2, 9]]).cuda()
+    assert calls.kv_copy_blocks(a, pairs) and calls.kv_copy_blocks(iter(b), pairs) is None
+    ops.kv_copy_blocks(b, pairs.t().contiguous().t())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for bad in [(q.cpu(), kp, vp, tables, ctx, 0.1), (q, kp, vp, tables.int(), ctx, 0.1), (q, kp, vp, tables, ctx[:3], 0.1),
+                (q, kp, kp[:1], tables, ctx, 0.1), (q, kp, vp, tables, ctx, "x"), (None, kp, vp, tables, ctx, 0.1), (q,)]:
+        assert calls.kv4_paged_decode(*bad) is None
+    assert calls.kv4_gather_blocks(kp, vp, ids, "d", nat.MI_F16, ctx, True) is None
+    assert ops.read_status() == 0
+
+
 # ---------------------------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------------------------
