@@ -46,41 +46,51 @@ template <typename T> struct Raw8 {
   }
 };
 
-// Smallest and largest of a group spread over the two lanes of `pair`; NaN where there is one.
+// Smallest and largest of a group spread over two consecutive lanes, NaN where there is one: K's in the first
+// of the two, V's in the second (a whole warp calls).
 template <typename T>
-__device__ __forceinline__ void kv4_range(const Raw8<T> (&x)[2], unsigned pair, float& lo, float& hi) {
+__device__ __forceinline__ void kv4_range(const Raw8<T> (&k)[2], const Raw8<T> (&v)[2], bool second, float& lo, float& hi) {
   if constexpr (sizeof(T) == 2) {
     // two values an instruction; (lo, -hi) as one pair that a minimum reduces
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    const T2* p = reinterpret_cast<const T2*>(x[0].w);
-    const T2* q = reinterpret_cast<const T2*>(x[1].w);
-    T2 least = __hmin2_nan(p[0], q[0]), most = __hmax2_nan(p[0], q[0]);
+    auto least_most = [](const Raw8<T> (&x)[2]) {
+      const T2* p = reinterpret_cast<const T2*>(x[0].w);
+      const T2* q = reinterpret_cast<const T2*>(x[1].w);
+      T2 least = __hmin2_nan(p[0], q[0]), most = __hmax2_nan(p[0], q[0]);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      least = __hmin2_nan(least, __hmin2_nan(p[i], q[i]));
-      most = __hmax2_nan(most, __hmax2_nan(p[i], q[i]));
-    }
-    most = __hneg2(most);
-    const uint32_t a = *reinterpret_cast<const uint32_t*>(&least), b = *reinterpret_cast<const uint32_t*>(&most);
-    const uint32_t low = __byte_perm(a, b, 0x5410), high = __byte_perm(a, b, 0x7632);
-    T2 both = __hmin2_nan(*reinterpret_cast<const T2*>(&low), *reinterpret_cast<const T2*>(&high));
-    const uint32_t other = __shfl_xor_sync(pair, *reinterpret_cast<const uint32_t*>(&both), 1);
-    both = __hmin2_nan(both, *reinterpret_cast<const T2*>(&other));
+      for (int i = 1; i < 4; ++i) {
+        least = __hmin2_nan(least, __hmin2_nan(p[i], q[i]));
+        most = __hmax2_nan(most, __hmax2_nan(p[i], q[i]));
+      }
+      most = __hneg2(most);
+      const uint32_t a = *reinterpret_cast<const uint32_t*>(&least), b = *reinterpret_cast<const uint32_t*>(&most);
+      const uint32_t low = __byte_perm(a, b, 0x5410), high = __byte_perm(a, b, 0x7632);
+      const T2 both = __hmin2_nan(*reinterpret_cast<const T2*>(&low), *reinterpret_cast<const T2*>(&high));
+      return *reinterpret_cast<const uint32_t*>(&both);
+    };
+    const uint32_t kr = least_most(k), vr = least_most(v);
+    const uint32_t own = second ? vr : kr;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, second ? kr : vr, 1);
+    const T2 both = __hmin2_nan(*reinterpret_cast<const T2*>(&own), *reinterpret_cast<const T2*>(&other));
     lo = Elem<T>::to_f(both.x);
     hi = -Elem<T>::to_f(both.y);
   } else {
-    lo = hi = x[0].at(0);
-    float poison = 0.f;
+    float l[2], h[2], poison[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float f = x[i >> 3].at(i & 7);
-      lo = fminf(lo, f);
-      hi = fmaxf(hi, f);
-      poison = fmaf(f, 0.f, poison);  // NaN from a NaN (or an infinity)
+    for (int t = 0; t < 2; ++t) {
+      l[t] = h[t] = (t ? v : k)[0].at(0);
+      poison[t] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float f = (t ? v : k)[i >> 3].at(i & 7);
+        l[t] = fminf(l[t], f);
+        h[t] = fmaxf(h[t], f);
+        poison[t] = fmaf(f, 0.f, poison[t]);  // NaN from a NaN (or an infinity)
+      }
     }
-    lo = fminf(lo, __shfl_xor_sync(pair, lo, 1));
-    hi = fmaxf(hi, __shfl_xor_sync(pair, hi, 1));
-    lo += poison + __shfl_xor_sync(pair, poison, 1);
+    const float nan = (second ? poison[1] : poison[0]) + __shfl_xor_sync(0xffffffffu, second ? poison[0] : poison[1], 1);
+    lo = fminf(second ? l[1] : l[0], __shfl_xor_sync(0xffffffffu, second ? l[0] : l[1], 1)) + nan;
+    hi = fmaxf(second ? h[1] : h[0], __shfl_xor_sync(0xffffffffu, second ? h[0] : h[1], 1));
   }
 }
 
@@ -93,25 +103,28 @@ __device__ __forceinline__ float div15(float x) {
   return fmaf(fmaf(-15.f, q, x), r, q);
 }
 
-// A group's parameters from its smallest and largest value, and what its quotients need.
-struct Kv4Scale {
-  float m, s;
-  float inv, s16;  // 1 / (16 s) within 2^-23, 16 s
-  uint32_t word;   // (s, m) as a page holds them
-  bool any;        // false: all codes are 0
-  bool fast;       // s is far from the ends of fp32's range
-};
-__device__ __forceinline__ Kv4Scale kv4_scale(float lo, float hi) {
-  Kv4Scale g;
+// A group's parameter word (s, m) from its smallest and largest value.
+__device__ __forceinline__ uint32_t kv4_word(float lo, float hi) {
   const uint32_t mb = bf16_bits(lo);
-  g.m = __uint_as_float(mb << 16);
-  const uint32_t sb = bf16_bits(div15(hi - g.m));
-  g.s = __uint_as_float(sb << 16);
+  const uint32_t sb = bf16_bits(div15(hi - __uint_as_float(mb << 16)));
   // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
   const bool spoiled = (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u;
   // hi - m can be negative (m rounded up past a constant group): s <= 0 then, and all codes are 0.
-  g.any = !spoiled && g.s > 0.f;
-  g.word = spoiled ? 0x7fc00000u : (mb << 16) | (g.any ? sb : 0u);
+  return spoiled ? 0x7fc00000u : (mb << 16) | (sb & 0x8000u ? 0u : sb);
+}
+
+// What a group's quotients need.
+struct Kv4Scale {
+  float m, s;
+  float inv, s16;  // 1 / (16 s) within 2^-23, 16 s
+  bool any;        // false: all codes are 0
+  bool fast;       // s is far from the ends of fp32's range
+};
+__device__ __forceinline__ Kv4Scale kv4_scale(uint32_t word) {
+  Kv4Scale g;
+  g.m = kv4_min(word);
+  g.s = kv4_step(word);
+  g.any = g.s > 0.f;
   g.fast = g.s >= 0x1p-110f && g.s <= 0x1p110f;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(g.inv) : "f"(g.s));
   g.inv *= 0.0625f;
@@ -137,28 +150,43 @@ __device__ __forceinline__ uint32_t kv4_code_slow(const Kv4Scale& g, float d) {
   return (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(d, g.s)), 0.f), 15.f);
 }
 
-// Quantise a group spread over two consecutive lanes (twice eight values each): this lane's codes, eight a
-// word, and the group's parameter word.  `pair` is the mask of the two lanes.
+// Quantise a group of K and one of V, both spread over two consecutive lanes (twice eight values each), by a
+// whole warp: this lane's codes of both, eight a word, and the parameter word of K in the first of the two
+// lanes (`second` false), of V in the other: each lane works out one and is told the other.
 template <typename T>
-__device__ __forceinline__ void kv4_quantise(const Raw8<T> (&x)[2], unsigned pair, uint32_t (&code)[2], uint32_t& word) {
+__device__ __forceinline__ void kv4_quantise(const Raw8<T> (&k)[2], const Raw8<T> (&v)[2], bool second, uint32_t (&kc)[2],
+                                             uint32_t (&vc)[2], uint32_t& word) {
   float lo, hi;
-  kv4_range<T>(x, pair, lo, hi);
-  const Kv4Scale g = kv4_scale(lo, hi);
-  word = g.word;
-  code[0] = code[1] = 0u;
-  if (!g.any) return;
-  if (g.fast) {
+  kv4_range<T>(k, v, second, lo, hi);
+  word = kv4_word(lo, hi);
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);
+  const Kv4Scale gk = kv4_scale(second ? other : word), gv = kv4_scale(second ? word : other);
+  const bool odd = (gk.any && !gk.fast) || (gv.any && !gv.fast);
+  if (!__any_sync(0xffffffffu, odd)) {
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
+      kc[n] = vc[n] = 0u - kKv4CodeBase * 0x11111111u;  // less the digits' common part
 #pragma unroll
-      for (int i = 0; i < 8; ++i) code[n] += kv4_code(g, x[n].less(i, g.m)) << (4 * i);
-      code[n] -= kKv4CodeBase * 0x11111111u;  // the digits' common part
+      for (int i = 0; i < 8; ++i) {
+        kc[n] += kv4_code(gk, k[n].less(i, gk.m)) << (4 * i);
+        vc[n] += kv4_code(gv, v[n].less(i, gv.m)) << (4 * i);
+      }
+      if (!gk.any) kc[n] = 0u;
+      if (!gv.any) vc[n] = 0u;
     }
-  } else {
+    return;
+  }
+  auto digit = [](const Kv4Scale& g, float d) {
+    return !g.any ? 0u : g.fast ? kv4_code(g, d) - kKv4CodeBase : kv4_code_slow(g, d);
+  };
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < 2; ++n) {
+    kc[n] = vc[n] = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) code[n] |= kv4_code_slow(g, x[n].at(i) - g.m) << (4 * i);
+    for (int i = 0; i < 8; ++i) {
+      kc[n] |= digit(gk, k[n].at(i) - gk.m) << (4 * i);
+      vc[n] |= digit(gv, v[n].at(i) - gv.m) << (4 * i);
+    }
   }
 }
 
@@ -179,8 +207,8 @@ __device__ __forceinline__ uint32_t kv4_quantise_warp(const float (&x)[E], uint3
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     poison += __shfl_xor_sync(0xffffffffu, poison, o);
   }
-  const Kv4Scale g = kv4_scale(lo + poison, hi);
-  word = g.word;
+  word = kv4_word(lo + poison, hi);
+  const Kv4Scale g = kv4_scale(word);
   uint32_t code = 0;
   if (g.any) {
 #pragma unroll
