@@ -585,7 +585,8 @@ def kv4_scatter(
     v_pool: torch.Tensor,
 ) -> None:
     """``kv_scatter`` into 4-bit pools: token i = src[token_rows[i], :, token_positions[i], :] of K and V is
-    quantised into slot slot_mapping[i].  key/value: [B, H, L, D], or [B, H, D] with both index tensors None."""
+    quantised into slot slot_mapping[i].  key/value: [B, H, L, D], or [B, H, D] with both index tensors None.
+    Slots must be distinct: two tokens of one slot would leave a mixture of both."""
     if token_rows is None and token_positions is None and nat.calls().kv4_append(key, value, slot_mapping, k_pool, v_pool):
         return
     device = _require_cuda("kv4_scatter", key, value, slot_mapping, k_pool, v_pool, token_rows, token_positions)
@@ -735,8 +736,11 @@ def kv4_paged_decode(
         new = (key_new.data_ptr(), value_new.data_ptr(), _A2(*key_new.stride()[:2]), slot_mapping.data_ptr())
     if out is None:
         out = torch.empty((b, hq * d), dtype=query.dtype, device=device)
-    elif out.shape != (b, hq * d) or out.dtype != query.dtype or out.stride(-1) != 1:
+    elif (out.shape != (b, hq * d) or out.dtype != query.dtype or out.stride(-1) != 1
+          or b > 1 and out.stride(0) < hq * d):
         raise ValueError(f"out must be [{b}, {hq * d}] {query.dtype} with contiguous rows")
+    if ws is not None and not ws.is_contiguous():
+        raise ValueError("ws must be contiguous")
     if b == 0:
         return out
     need = nat.load().mi_kv4_paged_decode_workspace_size(b, hq, h, d, width, bs, code)
@@ -809,6 +813,8 @@ def kv4_qk_norm_rope(
                          f"cos {tuple(c2.shape)}, sin {tuple(s2.shape)}, {slots.numel()} slots and pools of {h} heads")
     if any(t.dtype != q.dtype for t in (k, v, q_weight, k_weight, cos, sin)):
         raise ValueError(f"every dense operand must be {q.dtype}")
+    if any(w.shape != (d,) or not w.is_contiguous() for w in (q_weight, k_weight)):
+        raise ValueError(f"q_weight {tuple(q_weight.shape)} and k_weight {tuple(k_weight.shape)} must be contiguous [{d}]")
     q_out = torch.empty((tokens, num_q_heads, d), dtype=q.dtype, device=device)
     _launch(device, "mi_kv4_qk_norm_rope", q2.data_ptr(), q2.stride(0), k2.data_ptr(), k2.stride(0), v2.data_ptr(),
             v2.stride(0), q_weight.data_ptr(), k_weight.data_ptr(), c2.data_ptr(), s2.data_ptr(), c2.stride(0), tokens,

@@ -655,6 +655,24 @@ def test_the_ordinary_call_and_the_general_one_agree():
     assert ops.read_status() == 0
 
 
+def test_weights_outputs_and_workspaces_of_another_form_are_refused():
+    """Each would be read or written as if it were contiguous [D], distinct rows or a plain run of bytes."""
+    d, hq, h, bs, n = 64, 4, 2, 16, 3
+    x = torch.zeros((2, hq * d), dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(2 * d, dtype=torch.bfloat16, device="cuda")
+    cos, slots = x[:, :d], torch.tensor([0, 1]).cuda()
+    pools = [torch.zeros((n, h, ops.kv4_page_bytes(bs, d)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for qw, kw in [(w[:d], w[: d // 2]), (w[:d], w[::2]), (w[::2], w[:d]), (w[:d], w[:d, None])]:
+        with pytest.raises(ValueError, match="weight"):
+            ops.kv4_qk_norm_rope(x, x[:, : h * d], x[:, : h * d], qw, kw, cos, cos, 1e-6, hq, h, slots, *pools)
+    q, ctx = x.view(2, hq, d), torch.ones(2, dtype=torch.long, device="cuda")
+    tables = torch.ones((2, 40), dtype=torch.long, device="cuda")
+    with pytest.raises(ValueError, match="out"):
+        ops.kv4_paged_decode(q, *pools, tables, ctx, 1.0, out=x[:1].expand(2, hq * d))
+    with pytest.raises(ValueError, match="ws"):
+        ops.kv4_paged_decode(q, *pools, tables, ctx, 1.0, ws=torch.zeros(1 << 25, dtype=torch.uint8, device="cuda")[::2])
+
+
 # ---------------------------------------------------------------------------------------------
 # refusals
 # ---------------------------------------------------------------------------------------------
