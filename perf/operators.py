@@ -18,7 +18,6 @@ of a group holds value 2i in its low and value 2i + 1 in its high four bits), th
 * ``copy``: pages copied inside every layer's pools (a fork's private last page, a compaction).
 """
 
-import functools
 import sys
 from pathlib import Path
 
@@ -31,7 +30,6 @@ GROUP = 32
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 
 
-@functools.lru_cache(maxsize=1)
 def _ops():
     package = str(Path(__file__).resolve().parents[1] / "mini-infra-qwen3_b200")
     if package not in sys.path:
