@@ -5,7 +5,7 @@
 //
 // Tensor-core kernel (16-bit types, head_dim 64/128, block size 16/32, at most 8 query heads per KV
 // head).  With k = m + s c per group g of 32 values,
-//     q.k_t = sum_g s_tg (q_g . c_tg) + m_tg sum(q_g),     o = sum_t (p_t s_tg) c_tg + p_t m_tg,
+//     q.k_t = sum_g s_tg (q_g . c_tg) + m_tg sum(q_g),     o = sum_t (p_t s_tg) (c_tg - 8) + p_t (m_tg + 8 s_tg),
 // so the codes themselves are the MMA operands and the steps and minima enter once per token and group:
 // there is no pass that dequantises.  A code is masked out of its word straight into a half: c in bits
 // 0-3 of a half is the subnormal c * 2^-24, in bits 4-7 it is 16 c * 2^-24, both exact, so one AND makes
@@ -20,7 +20,14 @@
 //     product in fp16's upper range, so rounding costs at most 2^-11 of a weight (a group whose step is below
 //     2^-25 of its token's widest loses more of its own); an fp16 model, whose output has as many bits,
 //     carries the rounding's remainder in a second fp16 operand.
-//   * Scores, sums, the minimum terms and O are fp32.
+//   * Scores, sums, the minimum terms and O are fp32.  An output of a long flat row is small beside sum p s c
+//     (300 times smaller over 32,768 tokens) and that sum an MMA accumulator's, which rounds towards zero at every
+//     step: hence the codes less 8, by an MMA with -8 in place of the codes, and hence O outside the
+//     accumulators, which hold the sum of 16 or 32 tokens, exact or nearly, and are added to it with a
+//     rounding to nearest.  Relative errors of an fp16 model (rounding its output alone 2.1e-4), 900 rows of
+//     32,768 tokens: 2.3e-2 with whole codes summed in the accumulators, 9.2e-4 with the codes less 8, 2.2e-4
+//     as it is.  It costs 5 to 22 % of the time (64 rows of 16,384, bf16: 217 -> 228 us at 32/8 heads, 241 -> 287 at
+//     64/8; fp16: 250 -> 295, 286 -> 350).
 // Persistent CTAs, three a SM: a producer warp brings whole pages (all heads of a block in one bulk copy for
 // K and one for V) into a ring of steps of 32 tokens x 4 KV heads (or 64 x 2, 128 x 1), 4 consumer warps each
 // take a (KV head, 32 tokens) of a step.  The sequences' steps form one stream that the CTAs share in equal
@@ -391,11 +398,19 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
   constexpr int kSets = 2 / SH;
   constexpr int kTilePage = BS == 16 ? 2 * HB * S::kPageBytes : 0;
   constexpr int kTileTok = BS == 16 ? 0 : 16;
+  constexpr int kTileStep = kTilePage + kTileTok * 16;  // from a tile's codes to the next one's
   const int my_tile = SH == 2 ? t >> 1 : 0;
   const uint32_t my_par = my_tile * (kTilePage + kTileTok * NG * 4) + kPar + r * NG * 4;
   // SH = 2: ones in the columns of the first tile, and of the second.  Products rather than masks: the
   // ALU pipe, where the codes are cut, is the busiest.
   const __half2 ones[2] = {__float2half2_rn(r < 4 ? 1.f : 0.f), __float2half2_rn(r < 4 ? 0.f : 1.f)};
+  auto masked = [&](uint32_t w, int i) {
+    if constexpr (SH == 1) return w;
+    const __half2 m = __hmul2(*reinterpret_cast<const __half2*>(&w), ones[i]);
+    return *reinterpret_cast<const uint32_t*>(&m);
+  };
+  // -8 in place of the codes, in their units: 2^-24 for rows r, 2^-20 for rows r + 8
+  constexpr uint32_t kEights[4] = {0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u};
 
   // What a warp knows of its place is kept in shared memory: the loop over the tokens needs the registers.
   struct Place {
@@ -484,8 +499,8 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
       unit[1] = __shfl_sync(0xffffffffu, mine_unit, 8 * t + 4);
     }
 
-    float o[D / 16][4];  // O^T: rows are values, columns 2t, 2t + 1
-    float z[NG][2];      // sum p m of this lane's tokens
+    float o[D / 16][4];  // O^T less z: rows are values, columns 2t, 2t + 1
+    float z[NG][2];      // sum p (m + 8 s) of this lane's tokens
     float l[2] = {0.f, 0.f};
     float ref[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -498,9 +513,10 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
       if (left > 0) {
         const uint8_t* k_unit = smem + st * S::kStageBytes + k_off;
         const uint32_t k_mat = smem_u32(k_unit) + mat_row;
-        const uint32_t v_mat = k_mat + HB * S::kPageBytes;
+        // V's matrices: as K's, or (SH = 2) the token octets of one group in both tiles
+        const uint32_t v_mat = k_mat + HB * S::kPageBytes + (SH == 1 ? 0 : (lane >> 4) * (kTileStep - BS * 16));
         const bool tail = left < kKv4Unit;  // nothing past the sequence's end counts, whatever the pages hold there
-#pragma unroll
+#pragma unroll 1  // unrolled, the second set's loads come forward and spill 200 bytes
         for (int n = 0; n < kSets; ++n) {
           // ---- scores: x[0..1] token r, x[2..3] token r + 8 of the set's tile; columns 2t, 2t + 1 ----
           float x[4], wide[2];
@@ -601,7 +617,7 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
               ref[c] = want;
             }
           }
-          // ---- O^T += V^T (p s)^T, z += p m ----
+          // ---- O^T += (V^T - 8) (p s)^T, z += p (m + 8 s) ----
           l[0] += p[0] + p[2];
           l[1] += p[1] + p[3];
           const uint8_t* v_par = k_unit + my_par + n * (kTilePage + kTileTok * NG * 4) + HB * S::kPageBytes;
@@ -618,49 +634,55 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
           }
 #pragma unroll
           for (int gp = 0; gp < NG / 2; ++gp) {
-            uint32_t pb[2][kTwo ? 4 : 2];  // p s of the two groups as B operands (and what fp16 left of it)
+            uint32_t c[4];  // codes: SH = 1 of both groups, SH = 2 of one group of both tiles
+            if constexpr (SH == 1) ldmatrix_x4_trans(v_mat + n * kTileStep + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int g = gp * 2 + j;
               const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
               const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
-              z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
-              z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
               const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
               const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
-              pb[j][0] = movmatrix_trans(h0);
-              pb[j][1] = movmatrix_trans(h1);
+              uint32_t pb[2], rest[2];  // p s as a B operand, and what fp16 left of it
+              pb[0] = movmatrix_trans(h0);
+              pb[1] = movmatrix_trans(h1);
               if constexpr (kTwo) {
                 const float2 g0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
                 const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                pb[j][2] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
-                pb[j][3] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
+                rest[0] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
+                rest[1] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
+                // 8 times what fp16 holds of p s: the remainders meet whole codes
+                z[g][0] = fmaf(8.f, g0.x, fmaf(8.f, g1.x, fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]))));
+                z[g][1] = fmaf(8.f, g0.y, fmaf(8.f, g1.y, fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]))));
+              } else {
+                const float c0 = fmaf(8.f, s0, m0), c1 = fmaf(8.f, s1, m1);
+                z[g][0] = fmaf(p[2], c1, fmaf(p[0], c0, z[g][0]));
+                z[g][1] = fmaf(p[3], c1, fmaf(p[1], c0, z[g][1]));
               }
-            }
+              if constexpr (SH == 2) ldmatrix_x4_trans(v_mat + g * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
-            for (int i = 0; i < SH; ++i) {
-              uint32_t c[4];
-              ldmatrix_x4_trans(v_mat + (n + i) * (kTilePage + kTileTok * 16) + gp * 2 * BS * 16, c[0], c[1], c[2], c[3]);
+              for (int half = 0; half < 2; ++half) {
+                // sum (c - 8) p s of these tokens, the remainders (whole codes) first; added to O with a rounding
+                float u[4];
+                uint32_t cd[SH][4];
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int g = gp * 2 + j;
-                uint32_t lo[4], hi[4];
-                kv4_operands(c[2 * j], lo);
-                kv4_operands(c[2 * j + 1], hi);
-                const uint32_t a0[4] = {lo[0], lo[1], hi[0], hi[1]};
-                const uint32_t a1[4] = {lo[2], lo[3], hi[2], hi[3]};
-                uint32_t b[kTwo ? 4 : 2];
-#pragma unroll
-                for (int e = 0; e < (kTwo ? 4 : 2); ++e) {
-                  const __half2 w = __hmul2(*reinterpret_cast<const __half2*>(&pb[j][e]), ones[i]);
-                  b[e] = SH == 1 ? pb[j][e] : *reinterpret_cast<const uint32_t*>(&w);
+                for (int i = 0; i < SH; ++i) {
+                  const int w = SH == 1 ? 2 * j : 2 * i;
+                  const uint32_t lo = half ? c[w] >> 8 : c[w], hi = half ? c[w + 1] >> 8 : c[w + 1];
+                  cd[i][0] = lo & 0x000f000fu, cd[i][1] = lo & 0x00f000f0u;
+                  cd[i][2] = hi & 0x000f000fu, cd[i][3] = hi & 0x00f000f0u;
                 }
-                Mma16816<__half>::run(o[2 * g], a0, b[0], b[1]);
-                Mma16816<__half>::run(o[2 * g + 1], a1, b[0], b[1]);
                 if constexpr (kTwo) {
-                  Mma16816<__half>::run(o[2 * g], a0, b[2], b[3]);
-                  Mma16816<__half>::run(o[2 * g + 1], a1, b[2], b[3]);
+                  Mma16816<__half>::zero(u, cd[0], masked(rest[0], 0), masked(rest[1], 0));
+                  if constexpr (SH == 2) Mma16816<__half>::run(u, cd[SH - 1], masked(rest[0], 1), masked(rest[1], 1));
+                  Mma16816<__half>::run(u, kEights, pb[0], pb[1]);
+                } else {
+                  Mma16816<__half>::zero(u, kEights, pb[0], pb[1]);
                 }
+#pragma unroll
+                for (int i = 0; i < SH; ++i) Mma16816<__half>::run(u, cd[i], masked(pb[0], i), masked(pb[1], i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[2 * g + half][e] += u[e];
               }
             }
           }
