@@ -94,8 +94,9 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_decode_generic_kernel(cons
       }
       x = warp_sum(x);
       const float m_new = fmaxf(m_run, x);
+      // fmaxf passes a NaN score by, its weight does not: the row becomes NaN wherever the token stands
       const float alpha = m_new == -INFINITY ? 1.f : exp2f(m_run - m_new);
-      const float pr = m_new == -INFINITY ? 0.f : exp2f(x - m_new);
+      const float pr = x == -INFINITY ? 0.f : exp2f(x - m_new);
       l_run = l_run * alpha + pr;
       m_run = m_new;
 #pragma unroll
@@ -122,12 +123,12 @@ __global__ void __launch_bounds__(kKv4Warps * 32) kv4_decode_generic_kernel(cons
   for (int w = 0; w < kKv4Warps; ++w) m_all = fmaxf(m_all, sm[w]);
   float o = 0.f, l = 0.f;
   for (int w = 0; w < kKv4Warps; ++w) {
-    const float f = sm[w] == -INFINITY ? 0.f : exp2f(sm[w] - m_all);
+    const float f = m_all == -INFINITY ? 1.f : exp2f(sm[w] - m_all);  // a warp of no tokens: 0, of sums 0
     l += f * sl[w];
     o += f * so[w][d];
   }
   T* dst = reinterpret_cast<T*>(a.out + b * a.out_sb) + (int64_t)hq * a.head_dim;
-  dst[d] = Elem<T>::from_f(l == 0.f ? 0.f : o / l);
+  dst[d] = Elem<T>::from_f(ctx == 0 ? 0.f : o / l);
 }
 
 constexpr int kKv4Consumers = 4;  // consumer warps of the tensor-core kernel's CTA
