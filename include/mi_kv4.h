@@ -9,7 +9,7 @@
  * Format.  The head_dim values of one token and KV head are cut into groups of MI_KV4_GROUP = 32.
  * A group x stands for m + s * c with bfloat16 minimum m and step s and codes c in 0..15:
  *     m = bf16(min x),  s = bf16((max x - m) / 15),  c = clamp(round((x - m) / s), 0, 15)
- * in fp32 arithmetic, rounding to nearest even; c = 0 where s = 0.  A group with an infinity or a NaN
+ * in fp32 arithmetic, rounding to nearest even; c = 0 where s = 0; a zero m is +0.  A group with an infinity or a NaN
  * (or whose m or s overflows bfloat16) is stored as m = NaN, s = 0: it reads back as NaN.
  *   pool   uint8 [num_blocks, num_kv_heads, mi_kv4_page_bytes(block_size, head_dim)], contiguous
  *   page   codes [head_dim/32, block_size, 16 bytes]: byte i of a group holds value 2i in its low and

@@ -105,7 +105,8 @@ __device__ __forceinline__ float div15(float x) {
 
 // A group's parameter word (s, m) from its smallest and largest value.
 __device__ __forceinline__ uint32_t kv4_word(float lo, float hi) {
-  const uint32_t mb = bf16_bits(lo);
+  uint32_t mb = bf16_bits(lo);
+  if (mb == 0x8000u) mb = 0u;  // a zero minimum has no sign: which of +0 and -0 a reduction keeps is its own affair
   const uint32_t sb = bf16_bits(div15(hi - __uint_as_float(mb << 16)));
   // A group that no finite (s, m) describes reads back as NaN (an infinite hi makes an infinite s or a NaN).
   const bool spoiled = (mb & 0x7f80u) == 0x7f80u || (sb & 0x7f80u) == 0x7f80u;

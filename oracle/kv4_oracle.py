@@ -1,7 +1,7 @@
 """The 4-bit paged cache in numpy, in 64 bits, from the definitions in ``include/mi_kv4.h``.
 
 A group of 32 values of one token and head: m = bf16(min), s = bf16(fp32((max - m) / 15)),
-c = clamp(round((x - m) / s), 0, 15); it stands for m + s * c.
+c = clamp(round((x - m) / s), 0, 15), a zero m being +0; it stands for m + s * c.
 """
 
 from __future__ import annotations
@@ -25,7 +25,7 @@ def quantise(x: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray]:
     x = np.asarray(x, dtype=np.float64)
     g = x.reshape(*x.shape[:-1], -1, GROUP)
     with np.errstate(all="ignore"):
-        m = bf16(g.min(-1).astype(np.float32))
+        m = bf16(g.min(-1).astype(np.float32)) + np.float32(0)  # a zero minimum is +0
         s = bf16(((g.max(-1) - m.astype(np.float64)) / 15).astype(np.float32))
         bad = ~np.isfinite(g).all(-1) | ~np.isfinite(m) | ~np.isfinite(s)
         s = np.where(s > 0, s, np.float32(0))
