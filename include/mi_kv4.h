@@ -84,7 +84,7 @@ int mi_kv4_qk_norm_rope(const void* q, int64_t q_row_stride, const void* k, int6
  * mi_kv4_paged_decode — mi_paged_decode over 4-bit pools: one query token per sequence attends to
  * positions [0, context_lens[b]) of its block table; arguments as there.  With k_new, v_new,
  * new_strides and slot_mapping the new tokens are quantised into the pools first.  A row with
- * context length 0 gets zeros.  What the pages hold past a context length is never used.  A block id
+ * context length 0 gets zeros.  A table row covers at most 2^31 - 1 tokens (MI_ERR_UNSUPPORTED).  What the pages hold past a context length is never used.  A block id
  * out of range reads the null block and sets MI_STATUS_BAD_BLOCK.  Softmax, sums and accumulators
  * are fp32.
  */

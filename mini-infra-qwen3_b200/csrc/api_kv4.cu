@@ -171,7 +171,7 @@ int mi_kv4_qk_norm_rope(const void* q, int64_t q_row_stride, const void* k, int6
 size_t mi_kv4_paged_decode_workspace_size(int64_t batch, int num_q_heads, int num_kv_heads, int head_dim,
                                           int64_t max_blocks_per_seq, int block_size, int dtype) {
   if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || max_blocks_per_seq <= 0 ||
-      mi_kv4_page_bytes(block_size, head_dim) == 0)
+      mi_kv4_page_bytes(block_size, head_dim) == 0 || max_blocks_per_seq > kMaxGrid / block_size)
     return 0;
   return mi::plan_kv4_decode(batch, num_q_heads, num_kv_heads, head_dim, max_blocks_per_seq, block_size, dtype)
       .ws_bytes;
@@ -197,6 +197,9 @@ int mi_kv4_paged_decode(const void* q, const int64_t* q_strides, const void* k_n
   if (max_blocks_per_seq < 1 || (batch > 1 && table_stride < max_blocks_per_seq))
     return fail(MI_ERR_INVALID, "block table needs at least one column (max_blocks=%lld, stride=%lld)",
                 (long long)max_blocks_per_seq, (long long)table_stride);
+  if (max_blocks_per_seq > kMaxGrid / block_size)  // tokens of a row are counted in 32 bits
+    return fail(MI_ERR_UNSUPPORTED, "block tables of %lld blocks of %d: more than 2^31 - 1 tokens a row",
+                (long long)max_blocks_per_seq, block_size);
   const int es = elem_size(dtype);
   if (!aligned(q, es) || !aligned(out, es)) return fail(MI_ERR_INVALID, "mi_kv4_paged_decode: misaligned operands");
   mi::Kv4DecodePlan plan =
