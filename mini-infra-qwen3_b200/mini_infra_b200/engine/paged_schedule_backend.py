@@ -115,7 +115,7 @@ class PagedScheduleBackend:
         tables = [self.kv_cache_manager.block_table(c.state.request.request_idx) for c in chunks]
         starts = [c.start for c in chunks]
         chunk_ids = [c.state.request.token_ids[c.start : c.end] for c in chunks]
-        if self.runner.warm_mixed_graph([], chunk_ids, tables, self.pool):  # a shape's first step captures
+        if self.runner.warm_mixed_graph([], chunk_ids, tables, self.pool, starts):  # a shape's first step captures
             # a graph replay of forward + sample + the chunks' store (in model_ms)
             mixed = self.runner.run_mixed_step([], [], [], chunk_ids, starts, tables, self.pool)
             next_tokens, model_ms, cache = mixed.prefill_tokens, mixed.model_ms, None
@@ -171,7 +171,7 @@ class PagedScheduleBackend:
         c_tables = [self.kv_cache_manager.block_table(c.state.request.request_idx) for c in chunks]
         starts = [c.start for c in chunks]
         chunk_ids = [c.state.request.token_ids[c.start : c.end] for c in chunks]
-        self.runner.warm_mixed_graph(d_tables, chunk_ids, c_tables, self.pool)  # first use of a shape: capture
+        self.runner.warm_mixed_graph(d_tables, chunk_ids, c_tables, self.pool, starts)  # first use of a shape: capture
         out = self.runner.run_mixed_step(
             d_tables, [s.generated[-1] for s in decoding], [s.cache_length for s in decoding], chunk_ids, starts,
             c_tables, self.pool)

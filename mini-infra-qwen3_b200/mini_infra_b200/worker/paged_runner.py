@@ -117,19 +117,21 @@ class PagedRunner(BaseModelRunner):
             self.mixed_graphs.release()
         self.mixed_graphs = None
 
-    def _mixed_key(self, decode_tables, chunk_token_ids, chunk_tables, pool):
+    def _mixed_key(self, decode_tables, chunk_token_ids, chunk_tables, pool, start_positions):
         g = self.mixed_graphs
         if (g is None or not chunk_token_ids or min(len(t) for t in chunk_token_ids) < 1
                 or g.kv_pools[0][0].data_ptr() != pool.kv_pools[0][0].data_ptr()):
             return None
+        history = None if start_positions is None else max(-(-int(s) // pool.block_size) for s in start_positions)
         return g.key_for(len(decode_tables), len(chunk_token_ids), padded_width(max(len(t) for t in chunk_token_ids)),
-                         max((len(t) for t in decode_tables), default=0), max(len(t) for t in chunk_tables))
+                         max((len(t) for t in decode_tables), default=0), max(len(t) for t in chunk_tables), history)
 
-    def warm_mixed_graph(self, decode_tables, chunk_token_ids, chunk_tables, pool) -> bool:
+    def warm_mixed_graph(self, decode_tables, chunk_token_ids, chunk_tables, pool, start_positions=None) -> bool:
         """Count a mixed step (no decode rows: a prefill step) of this shape and capture its graph
         when the set decides to (outside any step timing); True when a graph serves the step.
-        Only shapes counted here are served by graphs."""
-        key = self._mixed_key(decode_tables, chunk_token_ids, chunk_tables, pool)
+        Only shapes counted here are served by graphs.  start_positions: the chunks', by which graphs over a
+        4-bit pool are told apart (None: any that the chunks' tables allow)."""
+        key = self._mixed_key(decode_tables, chunk_token_ids, chunk_tables, pool, start_positions)
         return key is not None and self.mixed_graphs.consider(key)
 
     def warm_decode_graph(self, batch: int, max_blocks: int) -> None:
@@ -291,8 +293,9 @@ class PagedRunner(BaseModelRunner):
         lens = [len(t) for t in chunk_token_ids]
         if bp == 0 or min(lens) < 1:
             raise ValueError("a mixed step needs non-empty chunks")
-        key = self._mixed_key(decode_block_tables, chunk_token_ids, chunk_block_tables, pool)
-        if key is not None and self.mixed_graphs.has(key):
+        key = self._mixed_key(decode_block_tables, chunk_token_ids, chunk_block_tables, pool, start_positions)
+        key = key and self.mixed_graphs.serving(key)
+        if key is not None:
             return self._replay_mixed(key, decode_block_tables, last_tokens, positions, chunk_token_ids,
                                       start_positions, chunk_block_tables)
         if nd == 0:
