@@ -316,8 +316,11 @@ def paged_prefill(
     chunk_lens: torch.Tensor,
     scale: float,
     out: torch.Tensor | None = None,
+    ws: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """Chunked-prefill attention: query [B, L, Hq, D], key/value_chunk [B, L, H, D] -> out [B, L, Hq * D]."""
+    """Chunked-prefill attention: query [B, L, Hq, D], key/value_chunk [B, L, H, D] -> out [B, L, Hq * D].
+
+    ws: workspace of the call's own (bytes; None: the device's, which calls on one stream share)."""
     device = _require_cuda("paged_prefill", query, key_chunk, value_chunk, k_pool, v_pool, block_tables,
                            start_positions, chunk_lens, out)
     if k_pool is None:  # no history: the pools are never read
@@ -352,10 +355,11 @@ def paged_prefill(
     need = int(lib.mi_paged_prefill_workspace_size(b, length, hq, h, d, table_stride, bs, code))
     ws_ptr, ws_bytes = ctypes.c_void_p(0), 0
     if need:
-        ws = workspace(device, need, slot="prefill")
+        if ws is None:
+            ws = workspace(device, need, slot="prefill")
         base = ws.data_ptr()
         ws_ptr = ctypes.c_void_p((base + 255) & ~255)
-        ws_bytes = ws.numel() - ((base + 255) & ~255) + base
+        ws_bytes = ws.nbytes - ((base + 255) & ~255) + base
     rc = lib.mi_paged_prefill(
         _ptr(query), nat.i64_array([query.stride(0), query.stride(1), query.stride(2)]), _ptr(key_chunk),
         _ptr(value_chunk), nat.i64_array([key_chunk.stride(0), key_chunk.stride(1), key_chunk.stride(2)]),
@@ -770,16 +774,24 @@ def kv4_paged_prefill(
 ) -> torch.Tensor:
     """``paged_prefill`` with its history in 4-bit pools: the history blocks are gathered as dense ones and
     attended to; the chunk's own K/V enter as they are, unquantised."""
-    if block_tables.numel() == 0:
-        return paged_prefill(query, key_chunk, value_chunk, None, None, block_tables, start_positions, chunk_lens, scale,
-                             out=out)
-    d = query.shape[-1]
-    key, value = kv4_gather_blocks(k_pool, v_pool, block_tables, d, query.dtype, lengths=start_positions,
-                                   fill_past=False)
-    b, nb = block_tables.shape
-    dense = torch.arange(b * nb, device=query.device).view(b, nb)
-    return paged_prefill(query, key_chunk, value_chunk, key.flatten(0, 1), value.flatten(0, 1), dense, start_positions,
-                         chunk_lens, scale, out=out)
+    if query.ndim != 4 or key_chunk.ndim != 4:
+        raise ValueError(f"query and chunk must be [B, L, heads, D], got {tuple(query.shape)} and {tuple(key_chunk.shape)}")
+    device = query.device
+    b, length, hq, d = query.shape
+    nb = block_tables.shape[-1] if block_tables.numel() else 0
+    key = value = None
+    tables, bs = block_tables, 1
+    if nb:
+        key, value = kv4_gather_blocks(k_pool, v_pool, block_tables, d, query.dtype, lengths=start_positions,
+                                       fill_past=False)
+        bs = key.shape[2]
+        key, value = key.flatten(0, 1), value.flatten(0, 1)
+        tables = torch.arange(block_tables.shape[0] * nb, device=device).view(-1, nb)
+    need = int(nat.load().mi_paged_prefill_workspace_size(b, length, hq, key_chunk.shape[2], d, nb, bs,
+                                                          dtype_code(query.dtype)))
+    ws = torch.empty(need + 256, dtype=torch.uint8, device=device) if need else None
+    return paged_prefill(query, key_chunk, value_chunk, key, value, tables, start_positions, chunk_lens, scale, out=out,
+                         ws=ws)
 
 
 def kv4_qk_norm_rope(
