@@ -777,6 +777,10 @@ def kv4_paged_prefill(
     if query.ndim != 4 or key_chunk.ndim != 4:
         raise ValueError(f"query and chunk must be [B, L, heads, D], got {tuple(query.shape)} and {tuple(key_chunk.shape)}")
     device = query.device
+    if device.type == "cuda" and device.index != torch.cuda.current_device():  # paged_prefill launches there
+        with torch.cuda.device(device):
+            return kv4_paged_prefill(query, key_chunk, value_chunk, k_pool, v_pool, block_tables, start_positions,
+                                     chunk_lens, scale, out)
     b, length, hq, d = query.shape
     nb = block_tables.shape[-1] if block_tables.numel() else 0
     key = value = None
