@@ -12,9 +12,10 @@ import ctypes
 import importlib.machinery
 import importlib.util
 import threading
+import warnings
 from pathlib import Path
 
-from mini_infra_b200.build import CALLS_PATH, LIB_PATH
+from mini_infra_b200.build import LIB_PATH, calls_path
 
 MI_F32, MI_BF16, MI_F16 = 0, 1, 2
 MI_OK, MI_ERR_INVALID, MI_ERR_CUDA, MI_ERR_UNSUPPORTED = 0, -1, -2, -3
@@ -113,23 +114,32 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+class _NoCalls:
+    """In place of the extension: takes no call, so that every one goes through ctypes to the same entry points."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 _calls = None
 
 
 def calls():
-    """The CPython extension over the library (``csrc/torch_calls.cpp``), loaded once."""
+    """The CPython extension over the library (``csrc/torch_calls.cpp``), loaded once; where there is none for this
+    Python and PyTorch, one that takes no call (with a warning: ctypes costs 8-20 us more a call)."""
     global _calls
     if _calls is None:
         load()
         with _lock:
-            if not CALLS_PATH.exists():
-                raise RuntimeError(f"{CALLS_PATH.name} not found at {CALLS_PATH}; build it with "
-                                   "`python -m mini_infra_b200.build`")
-            import torch  # noqa: F401  (its libraries resolve the extension's symbols)
-
-            loader = importlib.machinery.ExtensionFileLoader("_mi_calls", str(CALLS_PATH))
-            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mi_calls", loader))
-            loader.exec_module(module)
+            path = calls_path()  # imports PyTorch, whose libraries resolve the extension's symbols
+            loader = importlib.machinery.ExtensionFileLoader("_mi_calls", str(path))
+            try:
+                module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_mi_calls", loader))
+                loader.exec_module(module)
+            except ImportError as e:
+                warnings.warn(f"{path.name} cannot be loaded ({e}); the 4-bit operators go through ctypes.  "
+                              "Build it with `python -m mini_infra_b200.build`.", RuntimeWarning, stacklevel=3)
+                module = _NoCalls()
             _calls = module
     return _calls
 
