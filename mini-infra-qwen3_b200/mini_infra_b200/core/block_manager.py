@@ -185,8 +185,12 @@ class KVCacheManager:
     def free(self, request_idx: int) -> None:
         """Release the request's blocks (KeyError for a request holding no lease); a block that other
         requests share stays theirs."""
+        table = self._leases.pop(request_idx).table
+        if not self._sharers:  # nothing was forked
+            self.free_block_queue.free(table)
+            return
         own = []
-        for b in self._leases.pop(request_idx).table:
+        for b in table:
             others = self._sharers.pop(b, 0)
             if others > 1:
                 self._sharers[b] = others - 1
