@@ -776,6 +776,10 @@ def kv4_paged_prefill(
     attended to; the chunk's own K/V enter as they are, unquantised."""
     if query.ndim != 4 or key_chunk.ndim != 4:
         raise ValueError(f"query and chunk must be [B, L, heads, D], got {tuple(query.shape)} and {tuple(key_chunk.shape)}")
+    dense = (key_chunk, value_chunk) if out is None else (key_chunk, value_chunk, out)
+    if value_chunk.shape != key_chunk.shape or any(t.dtype != query.dtype for t in dense):
+        raise ValueError(f"chunk K {tuple(key_chunk.shape)} and V {tuple(value_chunk.shape)} must be alike and, as out, "
+                         f"{query.dtype}; got {', '.join(str(t.dtype) for t in dense)}")
     device = query.device
     if device.type == "cuda" and device.index != torch.cuda.current_device():  # paged_prefill launches there
         with torch.cuda.device(device):

@@ -57,3 +57,19 @@ def test_it_launches_with_its_tensors_device_current(monkeypatch, index, blocks)
     lens = meta(2, dtype=torch.long)
     assert ops.kv4_paged_prefill(query, chunk, chunk, None, None, tables, lens, lens, 1.0) == "out"
     assert seen == [index] * (1 + (blocks > 0)) and cuda.current == 0
+
+
+def test_operands_of_other_types_and_shapes_are_refused():
+    """Each would be read or written past its end, or as another type."""
+    x = lambda dtype=torch.bfloat16, length=5, heads=2: torch.zeros((2, length, heads, 64), dtype=dtype)  # noqa: E731
+    tables, lens = torch.zeros((2, 0), dtype=torch.long), torch.zeros(2, dtype=torch.long)
+    for k, v, out in [(x(torch.half), x(torch.half), None), (x(), x(torch.float), None), (x(torch.float), x(), None),
+                      (x(), x(length=4), None), (x(), x(heads=1), None),
+                      (x(), x(), torch.zeros((2, 5, 256), dtype=torch.half))]:
+        with pytest.raises(ValueError, match="alike"):
+            ops.kv4_paged_prefill(x(heads=4), k, v, None, None, tables, lens, lens, 1.0, out=out)
+    for q, k in [(x()[0], x()), (x(), x()[0])]:
+        with pytest.raises(ValueError, match="heads, D"):
+            ops.kv4_paged_prefill(q, k, k, None, None, tables, lens, lens, 1.0)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.kv4_paged_prefill(x(heads=4), x(), x(), None, None, tables, lens, lens, 1.0)
