@@ -20,14 +20,15 @@
 //     product in fp16's upper range, so rounding costs at most 2^-11 of a weight (a group whose step is below
 //     2^-25 of its token's widest loses more of its own); an fp16 model, whose output has as many bits,
 //     carries the rounding's remainder in a second fp16 operand.
-//   * Scores, sums, the minimum terms and O are fp32.  An output of a long flat row is small beside sum p s c
-//     (300 times smaller over 32,768 tokens) and that sum an MMA accumulator's, which rounds towards zero at every
-//     step: hence the codes less 8, by an MMA with -8 in place of the codes, and hence O outside the
-//     accumulators, which hold the sum of 16 or 32 tokens, exact or nearly, and are added to it with a
-//     rounding to nearest.  Relative errors of an fp16 model (rounding its output alone 2.1e-4), 900 rows of
-//     32,768 tokens: 2.3e-2 with whole codes summed in the accumulators, 9.2e-4 with the codes less 8, 2.2e-4
-//     as it is.  It costs 5 to 22 % of the time (64 rows of 16,384, bf16: 217 -> 228 us at 32/8 heads, 241 -> 287 at
-//     64/8; fp16: 250 -> 295, 286 -> 350).
+//   * Scores, sums, the minimum terms and O are fp32.  An output of a long row is small beside sum p s c (hundreds of
+//     times over 32,768 tokens of like weights), and an MMA rounds towards zero at every step, at the place of its
+//     largest term: hence the codes count from 8, their middle, and hence O stands outside the accumulators, which
+//     hold the sum of 16 or 32 tokens and are added to it with a rounding to nearest.  For bf16 the middle goes in by
+//     an MMA with -8 in place of the codes; that starts the sum at 128 p s, whose last place takes up to 1e-4 of a long
+//     row's output, so an fp16 model's operands are c - 8 themselves (one subtraction for two).  Relative
+//     errors, 900 rows of 32,768 tokens of like weights: with whole codes summed in the accumulators 2.3e-2 (fp16) and
+//     1.6e-2 (bf16), now 2.2e-4 and 1.7e-3, the outputs' rounding.  It takes 5 to 23 % of the time (64 rows of
+//     16,384, bf16: 217 -> 228 us at 32/8 heads, 241 -> 287 at 64/8; fp16: 250 -> 299, 286 -> 353).
 // Persistent CTAs, three a SM: a producer warp brings whole pages (all heads of a block in one bulk copy for
 // K and one for V) into a ring of steps of 32 tokens x 4 KV heads (or 64 x 2, 128 x 1), 4 consumer warps each
 // take a (KV head, 32 tokens) of a step.  The sequences' steps form one stream that the CTAs share in equal
@@ -167,6 +168,12 @@ __device__ __forceinline__ void kv4_operands(uint32_t w, uint32_t (&o)[4]) {
   const uint32_t w8 = w >> 8;
   o[2] = w8 & 0x000f000fu;
   o[3] = w8 & 0x00f000f0u;
+}
+
+// Two halves base + c, c a code, as c - 8 (exact).
+__device__ __forceinline__ uint32_t kv4_centred(uint32_t w, float base_and_8) {
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&w), __float2half2_rn(base_and_8));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
 
 template <int NG>
@@ -641,7 +648,10 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
             for (int j = 0; j < 2; ++j) {
               const int g = gp * 2 + j;
               const float s0 = kv4_step(vw[0][g]), s1 = kv4_step(vw[1][g]);
-              const float m0 = kv4_min(vw[0][g]), m1 = kv4_min(vw[1][g]);
+              // the value of code 8, the codes' middle
+              const float m0 = fmaf(8.f, s0, kv4_min(vw[0][g])), m1 = fmaf(8.f, s1, kv4_min(vw[1][g]));
+              z[g][0] = fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]));
+              z[g][1] = fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]));
               const float f[4] = {p[0] * s0, p[1] * s0, p[2] * s1, p[3] * s1};
               const uint32_t h0 = pack2<__half>(f[0], f[1]), h1 = pack2<__half>(f[2], f[3]);
               uint32_t pb[2], rest[2];  // p s as a B operand, and what fp16 left of it
@@ -652,31 +662,30 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
                 const float2 g1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
                 rest[0] = movmatrix_trans(pack2<__half>(f[0] - g0.x, f[1] - g0.y));
                 rest[1] = movmatrix_trans(pack2<__half>(f[2] - g1.x, f[3] - g1.y));
-                // 8 times what fp16 holds of p s: the remainders meet whole codes
-                z[g][0] = fmaf(8.f, g0.x, fmaf(8.f, g1.x, fmaf(p[2], m1, fmaf(p[0], m0, z[g][0]))));
-                z[g][1] = fmaf(8.f, g0.y, fmaf(8.f, g1.y, fmaf(p[3], m1, fmaf(p[1], m0, z[g][1]))));
-              } else {
-                const float c0 = fmaf(8.f, s0, m0), c1 = fmaf(8.f, s1, m1);
-                z[g][0] = fmaf(p[2], c1, fmaf(p[0], c0, z[g][0]));
-                z[g][1] = fmaf(p[3], c1, fmaf(p[1], c0, z[g][1]));
               }
               if constexpr (SH == 2) ldmatrix_x4_trans(v_mat + g * BS * 16, c[0], c[1], c[2], c[3]);
 #pragma unroll
               for (int half = 0; half < 2; ++half) {
-                // sum (c - 8) p s of these tokens, the remainders (whole codes) first; added to O with a rounding
+                // sum (c - 8) p s of these tokens, the remainders first; added to O with a rounding
                 float u[4];
                 uint32_t cd[SH][4];
 #pragma unroll
                 for (int i = 0; i < SH; ++i) {
                   const int w = SH == 1 ? 2 * j : 2 * i;
                   const uint32_t lo = half ? c[w] >> 8 : c[w], hi = half ? c[w + 1] >> 8 : c[w + 1];
-                  cd[i][0] = lo & 0x000f000fu, cd[i][1] = lo & 0x00f000f0u;
-                  cd[i][2] = hi & 0x000f000fu, cd[i][3] = hi & 0x00f000f0u;
+                  if constexpr (kTwo) {
+                    cd[i][0] = kv4_centred((lo & 0x000f000fu) | 0x64006400u, 1032.f);
+                    cd[i][1] = kv4_centred((lo & 0x00f000f0u) | 0x54005400u, 72.f);
+                    cd[i][2] = kv4_centred((hi & 0x000f000fu) | 0x64006400u, 1032.f);
+                    cd[i][3] = kv4_centred((hi & 0x00f000f0u) | 0x54005400u, 72.f);
+                  } else {
+                    cd[i][0] = lo & 0x000f000fu, cd[i][1] = lo & 0x00f000f0u;
+                    cd[i][2] = hi & 0x000f000fu, cd[i][3] = hi & 0x00f000f0u;
+                  }
                 }
                 if constexpr (kTwo) {
                   Mma16816<__half>::zero(u, cd[0], masked(rest[0], 0), masked(rest[1], 0));
                   if constexpr (SH == 2) Mma16816<__half>::run(u, cd[SH - 1], masked(rest[0], 1), masked(rest[1], 1));
-                  Mma16816<__half>::run(u, kEights, pb[0], pb[1]);
                 } else {
                   Mma16816<__half>::zero(u, kEights, pb[0], pb[1]);
                 }
@@ -729,7 +738,9 @@ __global__ void __launch_bounds__(kKv4SplitThreads, kKv4CtasPerSm) kv4_decode_sp
         for (int g = 0; g < NG; ++g) z[g][c] += __shfl_xor_sync(0xffffffffu, z[g][c], off);
       }
     }
-    auto value = [&](int g, int c, int i) { return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], i & 1 ? 0x1p20f : 0x1p24f, z[g][c]); };
+    auto value = [&](int g, int c, int i) {
+      return fmaf(o[2 * g + (i >> 1)][c + (i & 1) * 2], kTwo ? 1.f : i & 1 ? 0x1p20f : 0x1p24f, z[g][c]);
+    };
     // The rows' outputs where all of the sequence was here, else a partial: slot 0 the CTA's first, 1 its last.
     const int64_t b = pl.w.b;
     const int hb = pl.w.hb, pos = pl.w.pos, steps = pl.w.steps;

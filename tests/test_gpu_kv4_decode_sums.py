@@ -59,8 +59,8 @@ def sums_tolerance(q, k, v_pool, ids, want, n, scale, bs, dtype):
             + (2.0**-25 if dtype == "fp16" else 1e-30))
 
 
-@pytest.mark.parametrize("b,hq,h,d,bs,n,dtype", CASES)
-def test_long_flat_rows_keep_their_small_outputs(b, hq, h, d, bs, n, dtype):
+def long_rows(b, hq, h, d, bs, n, dtype, spread):
+    """(query, pools, tables): rows over the same pages, each in an order of its own."""
     g = torch.Generator(device="cuda").manual_seed(b + hq + d)
     rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
     pages = n // bs
@@ -68,8 +68,13 @@ def test_long_flat_rows_keep_their_small_outputs(b, hq, h, d, bs, n, dtype):
     vp = torch.zeros_like(kp)
     ops.kv4_scatter(rnd(n, h, d).to(DTYPES[dtype]), rnd(n, h, d).to(DTYPES[dtype]), None, None,
                     torch.arange(bs, bs + n).cuda(), kp, vp)
-    tables = 1 + torch.rand((b, pages), generator=g, device="cuda").argsort(dim=1)  # the same pages, in another order
-    q = (0.05 * rnd(b, hq, d)).to(DTYPES[dtype])
+    tables = 1 + torch.rand((b, pages), generator=g, device="cuda").argsort(dim=1)
+    return (spread * rnd(b, hq, d)).to(DTYPES[dtype]), kp, vp, tables
+
+
+@pytest.mark.parametrize("b,hq,h,d,bs,n,dtype", CASES)
+def test_long_flat_rows_keep_their_small_outputs(b, hq, h, d, bs, n, dtype):
+    q, kp, vp, tables = long_rows(b, hq, h, d, bs, n, dtype, 0.05)
     scale = d**-0.5
     got = ops.kv4_paged_decode(q, kp, vp, tables, torch.full((b,), n).cuda(), scale)
     assert ops.read_status() == 0
@@ -82,3 +87,19 @@ def test_long_flat_rows_keep_their_small_outputs(b, hq, h, d, bs, n, dtype):
         tol = sums_tolerance(qi, k, vp, ids, want, n, scale, bs, dtype)
         err = np.abs(got[i].double().cpu().numpy().reshape(hq, d) - want)
         assert (err <= tol).all(), f"row {i}: {(err / tol).max():.2f} of the tolerance"
+
+
+@pytest.mark.parametrize("b,dtype", [(8, "fp16"), (8, "bf16"), (500, "fp16"), (500, "bf16")])
+def test_long_rows_of_unlike_weights_have_no_bias(b, dtype):
+    """The mean error of N outputs whose roundings are independent, each of a standard deviation of at most half a unit
+    / sqrt(3) of its output (bf16: and a quarter of that for the weights' own): six standard deviations of the mean."""
+    hq, h, d, bs, n = 8, 1, 128, 32, 32768
+    q, kp, vp, tables = long_rows(b, hq, h, d, bs, n, dtype, 1.0)
+    got = ops.kv4_paged_decode(q, kp, vp, tables, torch.full((b,), n).cuda(), d**-0.5)
+    kp, vp = kp.cpu().numpy(), vp.cpu().numpy()
+    rows = list(range(8)) if b == 8 else [0, 100, 200, 300, 400, 499]
+    want = np.stack([ko.decode(q[i : i + 1].double().cpu().numpy(), kp, vp, tables[i : i + 1].cpu().numpy(), [n], d**-0.5, bs)[0]
+                     for i in rows])
+    error = (got[rows].double().cpu().numpy() - want).mean() / np.sqrt((want**2).mean())
+    half = torch.finfo(DTYPES[dtype]).eps / 2
+    assert abs(error) <= 6 * 1.04 * half / np.sqrt(3) / np.sqrt(want.size)
