@@ -322,7 +322,9 @@ def paged_prefill(
 
     ws: workspace of the call's own (bytes; None: the device's, which calls on one stream share)."""
     device = _require_cuda("paged_prefill", query, key_chunk, value_chunk, k_pool, v_pool, block_tables,
-                           start_positions, chunk_lens, out)
+                           start_positions, chunk_lens, out, ws)
+    if ws is not None and not ws.is_contiguous():
+        raise ValueError("ws must be contiguous")
     if k_pool is None:  # no history: the pools are never read
         n, bs, h, d = 1, 1, int(key_chunk.shape[2]), int(key_chunk.shape[3])
         if block_tables.numel() != 0:

@@ -96,3 +96,17 @@ def test_two_streams_and_a_captured_graph_share_no_workspace(monkeypatch):
         torch.cuda.synchronize()
         assert torch.equal(outs[0], want[0]) and torch.equal(outs[1], want[1]) and torch.equal(again, want[0])
     assert ops.read_status() == 0
+
+
+def test_workspaces_of_another_form_are_refused():
+    q, k, v, kp, vp, tables, starts, lens, scale = case(1)
+    starts.zero_()
+    args = (q, k, v, None, None, tables[:, :0], starts, lens, scale)
+    with pytest.raises(ValueError, match="ws"):
+        ops.paged_prefill(*args, ws=torch.zeros(1 << 27, dtype=torch.uint8, device="cuda")[::2])
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        ops.paged_prefill(*args, ws=torch.zeros(1 << 20, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="workspace"):
+        ops.paged_prefill(*args, ws=torch.zeros(512, dtype=torch.uint8, device="cuda"))
+    want = ops.paged_prefill(*args)
+    assert torch.equal(ops.paged_prefill(*args, ws=torch.zeros(1 << 27, dtype=torch.uint8, device="cuda")), want)
