@@ -9,8 +9,8 @@
  * Format.  The head_dim values of one token and KV head are cut into groups of MI_KV4_GROUP = 32.
  * A group x stands for m + s * c with bfloat16 minimum m and step s and codes c in 0..15:
  *     m = bf16(min x),  s = bf16((max x - m) / 15),  c = clamp(round((x - m) / s), 0, 15)
- * in fp32 arithmetic, rounding to nearest even; c = 0 where s = 0; a zero m is +0.  A group with an infinity or a NaN
- * (or whose m or s overflows bfloat16) is stored as m = NaN, s = 0: it reads back as NaN.
+ * in fp32 arithmetic, rounding to nearest even; c = 0 where s = 0; a zero m is +0.  A group with an infinity or a
+ * NaN (or whose m or s overflows bfloat16) is stored as m = NaN, s = 0: it reads back as NaN.
  *   pool   uint8 [num_blocks, num_kv_heads, mi_kv4_page_bytes(block_size, head_dim)], contiguous
  *   page   codes [head_dim/32, block_size, 16 bytes]: byte i of a group holds value 2i in its low and
  *          value 2i + 1 in its high four bits; then parameters [block_size, head_dim/32] of (s, m),
@@ -57,12 +57,12 @@ int mi_kv4_store_chunks(const void* k_src, const void* v_src, const int64_t* k_s
 
 /*
  * mi_kv4_gather_blocks — blocks of both pools as dense ones: out[b, j] = values of block
- * block_ids[b * id_stride + j], rounded to dtype; k_out/v_out contiguous
+ * block_ids[b * id_stride + j], rounded to dtype (fp16 by way of fp32); k_out/v_out contiguous
  * [batch, blocks_per_row, block_size, num_kv_heads, head_dim], the layout of a dense pool of
  * batch * blocks_per_row blocks.  With lengths (NULL: all), row b's tokens at and past lengths[b] are
  * written as zeros, whatever the pages hold there, and the ids of blocks wholly past it are not read;
- * with fill_past == 0 those blocks are not written either (the attention reads none of them).  A block id out of range reads as zeros and sets
- * MI_STATUS_BAD_BLOCK.
+ * with fill_past == 0 those blocks are not written either (the attention reads none of them).  A block
+ * id out of range reads as zeros and sets MI_STATUS_BAD_BLOCK.
  */
 int mi_kv4_gather_blocks(const void* k_pool, const void* v_pool, const int64_t* block_ids, int64_t id_stride,
                          const int64_t* lengths, int fill_past, int64_t batch, int64_t blocks_per_row, void* k_out,
@@ -84,7 +84,8 @@ int mi_kv4_qk_norm_rope(const void* q, int64_t q_row_stride, const void* k, int6
  * mi_kv4_paged_decode — mi_paged_decode over 4-bit pools: one query token per sequence attends to
  * positions [0, context_lens[b]) of its block table; arguments as there.  With k_new, v_new,
  * new_strides and slot_mapping the new tokens are quantised into the pools first.  A row with
- * context length 0 gets zeros.  A table row covers at most 2^31 - 1 tokens (MI_ERR_UNSUPPORTED).  What the pages hold past a context length is never used.  A block id
+ * context length 0 gets zeros.  A table row covers at most 2^31 - 1 tokens (MI_ERR_UNSUPPORTED).  What
+ * the pages hold past a context length is never used.  A block id
  * out of range reads the null block and sets MI_STATUS_BAD_BLOCK.  Softmax, sums and accumulators
  * are fp32.
  */

@@ -33,9 +33,10 @@
 // K and one for V) into a ring of steps of 32 tokens x 4 KV heads (or 64 x 2, 128 x 1), 4 consumer warps each
 // take a (KV head, 32 tokens) of a step.  The sequences' steps form one stream that the CTAs share in equal
 // ranges; pieces of a sequence cut by a border are merged by the combine kernel.
-// Bound by HBM: 64 rows of up to 32,768 tokens, 32/8 heads, 1.36 GB of pages in 223 us, 6.3 TB/s, where a
-// copy reaches 6.55; run for seconds the power limit lowers the clocks and the ALU work of cutting codes shows
-// (266 us).  One CTA per (row, 1,024 tokens) instead took 260 us: its waves ended raggedly.
+// Bound by HBM: 64 rows of 32,768 tokens, 32/8 heads, bf16, 2.68 GB of pages in 454 us, 5.9 TB/s, where a copy
+// reaches 6.55; run for seconds the power limit lowers the clocks and the ALU work of cutting codes shows (64 rows of
+// up to 32,768: 234 us -> 270).  One CTA per (row, 1,024 tokens) took 260 us where equal ranges took 236: its waves
+// ended raggedly.
 //
 // Generic kernel (any type, head_dim, block size and group count): one CTA per (sequence, query head);
 // its warps take the pages in turn, a lane holding value lane of every group, with an online softmax in

@@ -219,7 +219,8 @@ __device__ __forceinline__ uint32_t kv4_quantise_warp(const float (&x)[E], uint3
   return code;
 }
 
-// The eight values that packed codes and a parameter word stand for, rounded once to T.
+// The eight values that packed codes and a parameter word stand for, rounded to T: bf16 and fp32 once, fp16 by way of
+// fp32 (the parameters are no halves), half a unit and 2^-24 of the value at most.
 template <typename T>
 __device__ __forceinline__ Raw8<T> kv4_values(uint32_t code, uint32_t par) {
   Raw8<T> v;
